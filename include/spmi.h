@@ -669,6 +669,74 @@ int spmi_bn_act_linear_bwd(const float* z, int64_t M, int64_t wi, int64_t wi_pad
 int spmi_bn_bwd_apply(const float* dy, const float* z, int64_t M, int64_t W, int64_t w_pad,
                       const float* stats, const float* sums, float* dz, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Layer norm of rows: y = (x - mean) r w + b with r = (variance + eps)^-1/2, the variance taken
+ * over the row's D values (1 <= D <= spmi_layer_norm_max_width()).  x and y are float32 or
+ * bfloat16 (`dtype`) with row strides in values (0 repeats one row; any alignment), w and b
+ * float32 [D] (NULL: ones, zeros); everything between is float32.  The framework has no
+ * counterpart in the reference for it: it is the normalisation of the GLRU decoder's layers.
+ *   stats   nullable, float32 [M, 2]: each row's mean and r, for the backward pass
+ *   bwd     g = gradient of y -> dx (nullable), dweight, dbias (nullable); the sums over rows are
+ *           taken in a fixed order (ws: spmi_layer_norm_bwd_workspace_bytes, needed for them only)
+ * ---------------------------------------------------------------------- */
+int64_t spmi_layer_norm_max_width(void);
+int spmi_layer_norm_fwd(const void* x, int dtype, int64_t ldx, int64_t M, int64_t D, const float* weight,
+                        const float* bias, float eps, void* y, int64_t ldy, float* stats, void* stream);
+size_t spmi_layer_norm_bwd_workspace_bytes(int64_t M, int64_t D);
+int spmi_layer_norm_bwd(const void* x, const void* g, int dtype, int64_t ldx, int64_t ldg, int64_t M, int64_t D,
+                        const float* weight, const float* stats, void* dx, int64_t lddx, float* dweight,
+                        float* dbias, void* ws, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Gated linear recurrence (the GLRU decoder): with z = gates[t, n, 0:H], c = gates[t, n, H:2H],
+ *   h_t = sigmoid(z) h_{t-1} + (1 - sigmoid(z)) c
+ * over T steps for N nodes, as one scan.  gates, h, g, dgates are float32 or bfloat16 (`dtype`)
+ * with strides in values along steps (_t) and nodes (_n), units contiguous; states are float32.
+ *   h0       nullable (zeros), [N, H] with row stride h0_n
+ *   active   nullable, one byte per step and node (strides in bytes): where it is 0 the state
+ *            passes unchanged and the gates are not used (their gradient is 0)
+ *   last     float32 [N, H]: the state after the last step (h0 if T = 0)
+ *   bwd      g, g_last (nullable: zeros) = gradients of h and last; h as the forward wrote it (not
+ *            read if T <= 1) -> dgates, dh0 (nullable, [N, H])
+ *   ws       the matching _workspace_bytes (0 for most sizes), aligned to 16 bytes
+ * spmi_gated_step is one step on rows of the node memory h_mem [nodes, H] (contiguous): row i
+ * belongs to node ids[i] (NULL: i); h_out float32 [M, H] gets the new states, h_before (nullable)
+ * the old ones; with mem_write they also replace the memory's rows.  Every row starts from the
+ * memory as it was before the call; of several rows that name one node the memory keeps the last.
+ * A row whose id is outside [0, nodes) comes out as NaN and is written nowhere else.
+ * ---------------------------------------------------------------------- */
+size_t spmi_gated_scan_fwd_workspace_bytes(int64_t T, int64_t N, int64_t H);
+size_t spmi_gated_scan_bwd_workspace_bytes(int64_t T, int64_t N, int64_t H);
+int spmi_gated_scan_fwd(const void* gates, int dtype, int64_t gates_t, int64_t gates_n, const float* h0, int64_t h0_n,
+                        const uint8_t* active, int64_t active_t, int64_t active_n, int64_t T, int64_t N, int64_t H,
+                        void* h, int64_t h_t, int64_t h_n, float* last, void* ws, size_t ws_bytes, void* stream);
+int spmi_gated_scan_bwd(const void* gates, int dtype, int64_t gates_t, int64_t gates_n, const float* h0, int64_t h0_n,
+                        const uint8_t* active, int64_t active_t, int64_t active_n, int64_t T, int64_t N, int64_t H,
+                        const void* h, int64_t h_t, int64_t h_n, const void* g, int64_t g_t, int64_t g_n,
+                        const float* g_last, int64_t gl_n, void* dgates, int64_t dg_t, int64_t dg_n, float* dh0,
+                        void* ws, size_t ws_bytes, void* stream);
+size_t spmi_gated_step_workspace_bytes(int64_t M, int64_t nodes);
+int spmi_gated_step(const void* gates, int dtype, int64_t ldg, float* h_mem, int64_t nodes, const int64_t* ids,
+                    int64_t M, int64_t H, float* h_out, float* h_before, int mem_write, void* ws, size_t ws_bytes,
+                    void* stream);
+
+/* ------------------------------------------------------------------------
+ * Projection in 8-bit integers, for serving (the 8-bit form of the Linear layers that
+ * spmi_gemm_rows and spmi_gemm_rows_bf16 run, spiro/dtdg/models/decoder/torch/simpleDecoder.py:43-46):
+ *   q = rint(x * (127 / m)), s = m / 127, m = the row's largest magnitude (at least 2^-120)
+ *   y = act(s_row * w_scale[n] * sum_k q[k] w[n, k] + bias[n])
+ * with the quotient and the product of q rounded to float32 and the sum exact (K <= 131072).  A
+ * row of x with a value that is not finite comes out as NaN (its q are 0, its scale NaN).
+ * spmi_quantize_rows_i8 gives q and s alone: applied to a weight [N, K] it makes w and w_scale.
+ * x and out are float32 or bfloat16; rows of x, w and out have strides in values and any alignment.
+ * ---------------------------------------------------------------------- */
+int spmi_quantize_rows_i8(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, int8_t* q, int64_t ldq,
+                          float* scale, void* stream);
+size_t spmi_linear_i8_workspace_bytes(int64_t M, int64_t K, int64_t N);
+int spmi_linear_i8(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, const int8_t* weight, int64_t ldw,
+                   const float* w_scale, int64_t N, const float* bias /*nullable*/, int act, float slope, void* out,
+                   int out_dtype, int64_t ldo, void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -127,6 +127,25 @@ _SIGNATURES = {
     "spmi_cell_fused_supported": (c_int, [c_i64, c_i64]),
     "spmi_cell_fused_fwd": (c_int, [c_int, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
                                     c_vp, c_i64, c_i64, c_vp, c_vp, c_int, c_vp, c_vp]),
+    "spmi_layer_norm_max_width": (c_i64, []),
+    "spmi_layer_norm_fwd": (c_int, [c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_f32, c_vp, c_i64, c_vp, c_vp]),
+    "spmi_layer_norm_bwd_workspace_bytes": (c_sz, [c_i64, c_i64]),
+    "spmi_layer_norm_bwd": (c_int, [c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_vp,
+                                    c_vp, c_vp, c_sz, c_vp]),
+    "spmi_gated_scan_fwd_workspace_bytes": (c_sz, [c_i64, c_i64, c_i64]),
+    "spmi_gated_scan_bwd_workspace_bytes": (c_sz, [c_i64, c_i64, c_i64]),
+    "spmi_gated_scan_fwd": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64,
+                                    c_vp, c_i64, c_i64, c_vp, c_vp, c_sz, c_vp]),
+    "spmi_gated_scan_bwd": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64,
+                                    c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_vp,
+                                    c_vp, c_sz, c_vp]),
+    "spmi_gated_step_workspace_bytes": (c_sz, [c_i64, c_i64]),
+    "spmi_gated_step": (c_int, [c_vp, c_int, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_int, c_vp, c_sz,
+                                c_vp]),
+    "spmi_quantize_rows_i8": (c_int, [c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp]),
+    "spmi_linear_i8_workspace_bytes": (c_sz, [c_i64, c_i64, c_i64]),
+    "spmi_linear_i8": (c_int, [c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_int, c_f32, c_vp,
+                               c_int, c_i64, c_vp, c_sz, c_vp]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -1,0 +1,74 @@
+// Small device helpers of the row and sequence kernels (norm.hip, scan.hip, gemm_i8.hip): values of
+// float or bfloat16 rows as float, and reductions over neighbouring lanes.
+#pragma once
+
+#include "common.h"
+
+namespace spmi {
+
+using bf16 = __bf16;
+
+// Four neighbouring values as float, from any address that is a multiple of the value's own size:
+// global memory accesses need no more alignment than that on gfx950 (the compiler emits one 16-
+// or 8-byte access), so rows of an odd width or stride take the same code as aligned ones.
+__device__ __forceinline__ void load4(const float* p, float (&v)[4]) { __builtin_memcpy(v, p, 16); }
+__device__ __forceinline__ void load4(const bf16* p, float (&v)[4]) {
+  bf16 t[4];
+  __builtin_memcpy(t, p, 8);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = static_cast<float>(t[i]);
+}
+__device__ __forceinline__ void store4(float* p, const float (&v)[4]) { __builtin_memcpy(p, v, 16); }
+__device__ __forceinline__ void store4(bf16* p, const float (&v)[4]) {
+  bf16 t[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t[i] = static_cast<bf16>(v[i]);  // rounds to nearest even
+  __builtin_memcpy(p, t, 8);
+}
+
+// The same for the last values of a row: `left` >= 1 of them exist, the others read as `fill`.
+template <typename T>
+__device__ __forceinline__ void load4_upto(const T* p, int left, float fill, float (&v)[4]) {
+  if (left >= 4) {
+    load4(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < left ? static_cast<float>(p[i]) : fill;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store4_upto(T* p, int left, const float (&v)[4]) {
+  if (left >= 4) {
+    store4(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (i < left) p[i] = static_cast<T>(v[i]);
+  }
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+
+// The sum (maximum) over groups of G neighbouring lanes, in every lane of the group.  Inside 16
+// lanes the partner's value comes with the instruction itself (data-parallel primitives: swaps
+// within four lanes, mirrors of 8 and of 16); only the last two steps go through LDS hardware.
+// Every lane adds the same pairs, so all lanes hold the same bits.
+template <int G, typename Op>
+__device__ __forceinline__ float group_reduce(float v, Op op) {
+  if constexpr (G >= 2) v = op(v, dpp<0xB1>(v));   // lanes 1 0 3 2
+  if constexpr (G >= 4) v = op(v, dpp<0x4E>(v));   // lanes 2 3 0 1
+  if constexpr (G >= 8) v = op(v, dpp<0x141>(v));  // mirror of 8 lanes
+  if constexpr (G >= 16) v = op(v, dpp<0x140>(v)); // mirror of 16 lanes
+  if constexpr (G >= 32) v = op(v, __shfl_xor(v, 16, 64));
+  if constexpr (G >= 64) v = op(v, __shfl_xor(v, 32, 64));
+  return v;
+}
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+  return group_reduce<G>(v, [](float a, float b) { return a + b; });
+}
+
+}  // namespace spmi

@@ -1,0 +1,639 @@
+// The gated linear recurrence over a sequence, forward and backward, and its single step on the
+// node memory.  With gate logits z and candidates c (one projection's output, [.., 2H]):
+//
+//   a = sigmoid(z),  h_t = a_t h_{t-1} + (1 - a_t) c_t          per node and hidden unit
+//   backward, with e = the gradient that arrives at h_t from later steps:
+//   d = g_t + e,  dc = d (1 - a),  dz = d (h_{t-1} - c) a (1 - a),  e <- a d
+//
+// Nothing here depends on h but h itself, so both directions are a chain of maps v -> p v + q that
+// can be joined pairwise: a stretch of steps is one such map (p = product of the a, q = what the
+// stretch makes of zero).  Both are bound by memory (forward: two values in, one out per unit and
+// step; backward: four in, two out), and the design is about having enough loads in flight while
+// every value is read once:
+//  * many channels: a thread owns four neighbouring units of one node and walks the steps; the
+//    loads of several steps are issued together;
+//  * few channels (a long sequence of one or a few nodes): a workgroup is 8 strands of 32 lanes.
+//    A strand takes consecutive steps of a tile into registers, reduces them to its map, the maps
+//    meet in LDS, and each strand replays its steps from the registers with the right start: the
+//    inputs are still read once;
+//  * very few channels: the steps are also split over workgroups.  A first launch leaves the map
+//    of each split in a workspace (this reads the gates, and backward the gradients, a second
+//    time: mostly from the caches, since a problem of few channels is a small one), a second
+//    launch starts every split from the joined maps before it.  No workgroup waits for another.
+//
+// a and 1 - a are computed from exp(-|z|), so neither loses digits where it is small; the state, its
+// gradient and the maps are float32 whatever the storage type, and a state is rounded only when it
+// is stored.  Steps where a node is not active pass the state (and its gradient) on unchanged;
+// what stands in the gates there is loaded but never used.
+
+#include "lanes.h"
+
+namespace {
+
+using namespace spmi;
+
+constexpr int kThreads = 256;
+constexpr int kFwdSteps = 8;   // steps a thread holds in registers
+constexpr int kBwdSteps = 4;
+constexpr int kLanes = 32;     // shape of a workgroup over few channels: lanes x strands
+constexpr int kStrands = kThreads / kLanes;
+// Threads (of four units) from which the steps are walked by one thread each: one wave per SIMD.
+constexpr int64_t kManyLanes = 65536;
+// Up to this many steps there is nothing to share among the strands.
+constexpr int64_t kFewSteps = 16;
+constexpr int64_t kTargetGroups = 512;  // workgroups wanted before the steps are split further
+constexpr int64_t kMaxSplits = 256;
+
+struct ScanArgs {
+  const void* gates;   // [T, N, 2H]: z, then c
+  int64_t gates_t, gates_n;
+  const float* h0;     // nullable, [N, H]
+  int64_t h0_n;
+  const uint8_t* active;  // nullable, [T, N]
+  int64_t active_t, active_n;
+  void* h;             // [T, N, H]: written forward, read backward
+  int64_t h_t, h_n;
+  float* last;         // forward: [N, H]
+  const void* g;       // backward, nullable: gradient of h
+  int64_t g_t, g_n;
+  const float* g_last; // backward, nullable, [N, H]
+  int64_t gl_n;
+  void* dgates;        // backward, nullable, strides dg_t, dg_n
+  int64_t dg_t, dg_n;
+  float* dh0;          // backward, nullable, [N, H]
+  int64_t T, N;
+  int H, Hq;           // Hq = groups of four units per node
+  int64_t per_split;   // steps of a split
+  int splits;
+  float* maps;         // [splits][2][lanes][4]: p, then q
+};
+
+// e^-|z| to about one unit in the last place: the exponent's product with log2(e) is split so that
+// its rounding error is put back.
+__device__ __forceinline__ void gate_pair(float z, float& a, float& rest) {
+  const float m = -__builtin_fabsf(z);
+  const float y = m * 1.44269504f;
+  const float err = __builtin_fmaf(m, 1.44269504f, -y);
+  float e = __builtin_amdgcn_exp2f(y);
+  e = __builtin_fmaf(e, err * 0.693147181f, e);
+  e = m < -200.0f ? 0.0f : e;   // also -inf, where the error term is not a number
+  const float big = __builtin_amdgcn_rcpf(1.0f + e), small = e * big;
+  a = z >= 0.0f ? big : small;
+  rest = z >= 0.0f ? small : big;
+}
+
+// What a thread works on: four units of one node.
+struct Place {
+  bool there;
+  int64_t n;
+  int c, left;  // first unit, units from it to the end of the row
+  __device__ Place(const ScanArgs& p, int64_t lane) {
+    there = lane < p.N * p.Hq;
+    n = there ? lane / p.Hq : 0;
+    c = there ? static_cast<int>(lane - n * p.Hq) * 4 : 0;
+    left = p.H - c;
+  }
+};
+
+// Forward.  C lanes x S strands; MAPS: only the map of the split is wanted.
+template <typename T, int C, int S, bool MAPS>
+__global__ __launch_bounds__(kThreads) void scan_fwd_kernel(ScanArgs p) {
+  constexpr int L = kFwdSteps;
+  static_assert(C * S == kThreads, "lanes x strands");
+  __shared__ float4 meet[S > 1 ? 2 : 1][S][2][S > 1 ? C : 1];
+  const int lane = threadIdx.x % C, strand = threadIdx.x / C;
+  const int64_t channel = static_cast<int64_t>(blockIdx.x) * C + lane;
+  const Place at(p, channel);
+  const int split = blockIdx.y;
+  const int64_t lanes4 = p.N * p.Hq * 4;
+  const int64_t t_begin = split * p.per_split;
+  const int64_t t_end = t_begin + p.per_split < p.T ? t_begin + p.per_split : p.T;
+  const T* gates = static_cast<const T*>(p.gates) + at.n * p.gates_n + at.c;
+  const uint8_t* active = p.active ? p.active + at.n * p.active_n : nullptr;
+
+  float a[L][4], b[L][4];
+  bool on[L];
+  auto fetch = [&](int64_t t0) {
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      const int64_t t = t0 + strand * L + i;
+      on[i] = at.there && t < t_end;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) a[i][k] = b[i][k] = 0.0f;
+      if (on[i]) {
+        load4_upto(gates + t * p.gates_t, at.left, 0.0f, a[i]);
+        load4_upto(gates + t * p.gates_t + p.H, at.left, 0.0f, b[i]);
+        if (active) on[i] = active[t * p.active_t] != 0;
+      }
+    }
+  };
+  // z, c -> the step's map (a, (1 - a) c)
+  auto to_maps = [&]() {
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float keep, rest;
+        gate_pair(a[i][k], keep, rest);
+        b[i][k] = on[i] ? rest * b[i][k] : 0.0f;
+        a[i][k] = on[i] ? keep : 1.0f;
+      }
+  };
+
+  fetch(t_begin);
+
+  // the state the split starts from
+  float h[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  float prod[4] = {1.0f, 1.0f, 1.0f, 1.0f};  // MAPS
+  if constexpr (!MAPS) {
+    if (p.h0 && at.there) load4_upto(p.h0 + at.n * p.h0_n + at.c, at.left, 0.0f, h);
+    if constexpr (S > 1) {
+      if (split > 0) {
+        // each strand joins a share of the maps before this split, then the shares are joined
+        const int share = (split + S - 1) / S;
+        const int k0 = strand * share, k1 = k0 + share < split ? k0 + share : split;
+        float4 P = make_float4(1, 1, 1, 1), Q = make_float4(0, 0, 0, 0);
+        if (at.there) {
+          const float* m = p.maps + channel * 4;
+#pragma unroll 4
+          for (int k = k0; k < k1; ++k) {
+            const float4 pk = *reinterpret_cast<const float4*>(m + (2 * k) * lanes4);
+            const float4 qk = *reinterpret_cast<const float4*>(m + (2 * k + 1) * lanes4);
+            Q = make_float4(pk.x * Q.x + qk.x, pk.y * Q.y + qk.y, pk.z * Q.z + qk.z, pk.w * Q.w + qk.w);
+            P = make_float4(P.x * pk.x, P.y * pk.y, P.z * pk.z, P.w * pk.w);
+          }
+        }
+        meet[1][strand][0][lane] = P;
+        meet[1][strand][1][lane] = Q;
+        __syncthreads();
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          const float4 ps = meet[1][s][0][lane], qs = meet[1][s][1][lane];
+          h[0] = ps.x * h[0] + qs.x; h[1] = ps.y * h[1] + qs.y;
+          h[2] = ps.z * h[2] + qs.z; h[3] = ps.w * h[3] + qs.w;
+        }
+        // the first tile writes meet[0], the second meet[1] after a barrier of its own
+      }
+    }
+  }
+
+  int turn = 0;
+  for (int64_t t0 = t_begin; t0 < t_end; t0 += S * L) {
+    if (t0 != t_begin) fetch(t0);
+    to_maps();
+    float start[4];
+    if constexpr (S > 1) {
+      float P[4] = {1.0f, 1.0f, 1.0f, 1.0f}, Q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < L; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          P[k] *= a[i][k];
+          Q[k] = __builtin_fmaf(a[i][k], Q[k], b[i][k]);
+        }
+      meet[turn][strand][0][lane] = make_float4(P[0], P[1], P[2], P[3]);
+      meet[turn][strand][1][lane] = make_float4(Q[0], Q[1], Q[2], Q[3]);
+      __syncthreads();
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        if (s == strand) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) start[k] = h[k];
+        }
+        const float4 ps = meet[turn][s][0][lane], qs = meet[turn][s][1][lane];
+        h[0] = ps.x * h[0] + qs.x; h[1] = ps.y * h[1] + qs.y;
+        h[2] = ps.z * h[2] + qs.z; h[3] = ps.w * h[3] + qs.w;
+        if constexpr (MAPS) {
+          prod[0] *= ps.x; prod[1] *= ps.y; prod[2] *= ps.z; prod[3] *= ps.w;
+        }
+      }
+      turn ^= 1;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) start[k] = h[k];
+    }
+    if constexpr (!MAPS) {
+      T* out = static_cast<T*>(p.h) + at.n * p.h_n + at.c;
+#pragma unroll
+      for (int i = 0; i < L; ++i) {
+        const int64_t t = t0 + strand * L + i;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) start[k] = __builtin_fmaf(a[i][k], start[k], b[i][k]);
+        if (at.there && t < t_end) store4_upto(out + t * p.h_t, at.left, start);
+      }
+      if constexpr (S == 1) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) h[k] = start[k];
+      }
+    }
+  }
+
+  if (!at.there) return;
+  if constexpr (MAPS) {
+    if (strand == 0) {
+      float* m = p.maps + channel * 4 + static_cast<int64_t>(2 * split) * lanes4;
+      *reinterpret_cast<float4*>(m) = make_float4(prod[0], prod[1], prod[2], prod[3]);
+      *reinterpret_cast<float4*>(m + lanes4) = make_float4(h[0], h[1], h[2], h[3]);
+    }
+  } else if (split == p.splits - 1 && strand == 0) {
+    store4_upto(p.last + at.n * p.H + at.c, at.left, h);
+  }
+}
+
+// Backward, from the last step down: strand 0 has the latest steps of a tile, split 0 the latest
+// steps of all.
+template <typename T, int C, int S, bool MAPS>
+__global__ __launch_bounds__(kThreads) void scan_bwd_kernel(ScanArgs p) {
+  constexpr int L = kBwdSteps;
+  static_assert(C * S == kThreads, "lanes x strands");
+  __shared__ float4 meet[S > 1 ? 2 : 1][S][2][S > 1 ? C : 1];
+  const int lane = threadIdx.x % C, strand = threadIdx.x / C;
+  const int64_t channel = static_cast<int64_t>(blockIdx.x) * C + lane;
+  const Place at(p, channel);
+  const int split = blockIdx.y;
+  const int64_t lanes4 = p.N * p.Hq * 4;
+  // steps counted from the end: u = T - 1 - t
+  const int64_t u_begin = split * p.per_split;
+  const int64_t u_end = u_begin + p.per_split < p.T ? u_begin + p.per_split : p.T;
+  const T* gates = static_cast<const T*>(p.gates) + at.n * p.gates_n + at.c;
+  const T* g = static_cast<const T*>(p.g) + (p.g ? at.n * p.g_n + at.c : 0);
+  const T* h = static_cast<const T*>(p.h) + at.n * p.h_n + at.c;
+  const uint8_t* active = p.active ? p.active + at.n * p.active_n : nullptr;
+
+  float z[L][4], c[L][4], gv[L][4], hp[L][4];
+  bool on[L];
+  auto fetch = [&](int64_t u0) {
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      const int64_t u = u0 + strand * L + i, t = p.T - 1 - u;
+      on[i] = at.there && u < u_end;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) z[i][k] = c[i][k] = gv[i][k] = hp[i][k] = 0.0f;
+      if (on[i]) {
+        load4_upto(gates + t * p.gates_t, at.left, 0.0f, z[i]);
+        if (p.g) load4_upto(g + t * p.g_t, at.left, 0.0f, gv[i]);
+        if constexpr (!MAPS) {
+          load4_upto(gates + t * p.gates_t + p.H, at.left, 0.0f, c[i]);
+          if (t > 0) {
+            load4_upto(h + (t - 1) * p.h_t, at.left, 0.0f, hp[i]);
+          } else if (p.h0) {
+            load4_upto(p.h0 + at.n * p.h0_n + at.c, at.left, 0.0f, hp[i]);
+          }
+        }
+        if (active) on[i] = active[t * p.active_t] != 0;
+      }
+    }
+  };
+
+  fetch(u_begin);
+
+  float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  float prod[4] = {1.0f, 1.0f, 1.0f, 1.0f};  // MAPS
+  if constexpr (!MAPS) {
+    if (p.g_last && at.there) load4_upto(p.g_last + at.n * p.gl_n + at.c, at.left, 0.0f, e);
+    if constexpr (S > 1) {
+      if (split > 0) {
+        const int share = (split + S - 1) / S;
+        const int k0 = strand * share, k1 = k0 + share < split ? k0 + share : split;
+        float4 P = make_float4(1, 1, 1, 1), Q = make_float4(0, 0, 0, 0);
+        if (at.there) {
+          const float* m = p.maps + channel * 4;
+#pragma unroll 4
+          for (int k = k0; k < k1; ++k) {
+            const float4 pk = *reinterpret_cast<const float4*>(m + (2 * k) * lanes4);
+            const float4 qk = *reinterpret_cast<const float4*>(m + (2 * k + 1) * lanes4);
+            Q = make_float4(pk.x * Q.x + qk.x, pk.y * Q.y + qk.y, pk.z * Q.z + qk.z, pk.w * Q.w + qk.w);
+            P = make_float4(P.x * pk.x, P.y * pk.y, P.z * pk.z, P.w * pk.w);
+          }
+        }
+        meet[1][strand][0][lane] = P;
+        meet[1][strand][1][lane] = Q;
+        __syncthreads();
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          const float4 ps = meet[1][s][0][lane], qs = meet[1][s][1][lane];
+          e[0] = ps.x * e[0] + qs.x; e[1] = ps.y * e[1] + qs.y;
+          e[2] = ps.z * e[2] + qs.z; e[3] = ps.w * e[3] + qs.w;
+        }
+      }
+    }
+  }
+
+  int turn = 0;
+  for (int64_t u0 = u_begin; u0 < u_end; u0 += S * L) {
+    if (u0 != u_begin) fetch(u0);
+    float a[L][4], rest[L][4];
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        gate_pair(z[i][k], a[i][k], rest[i][k]);
+        if (!on[i]) a[i][k] = 1.0f;
+      }
+    float start[4];
+    if constexpr (S > 1) {
+      float P[4] = {1.0f, 1.0f, 1.0f, 1.0f}, Q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < L; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          P[k] *= a[i][k];
+          Q[k] = a[i][k] * (Q[k] + gv[i][k]);
+        }
+      meet[turn][strand][0][lane] = make_float4(P[0], P[1], P[2], P[3]);
+      meet[turn][strand][1][lane] = make_float4(Q[0], Q[1], Q[2], Q[3]);
+      __syncthreads();
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        if (s == strand) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) start[k] = e[k];
+        }
+        const float4 ps = meet[turn][s][0][lane], qs = meet[turn][s][1][lane];
+        e[0] = ps.x * e[0] + qs.x; e[1] = ps.y * e[1] + qs.y;
+        e[2] = ps.z * e[2] + qs.z; e[3] = ps.w * e[3] + qs.w;
+        if constexpr (MAPS) {
+          prod[0] *= ps.x; prod[1] *= ps.y; prod[2] *= ps.z; prod[3] *= ps.w;
+        }
+      }
+      turn ^= 1;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) start[k] = e[k];
+    }
+    if constexpr (!MAPS) {
+      T* out = static_cast<T*>(p.dgates) + at.n * p.dg_n + at.c;
+#pragma unroll
+      for (int i = 0; i < L; ++i) {
+        const int64_t u = u0 + strand * L + i, t = p.T - 1 - u;
+        float dz[4], dc[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float d = start[k] + gv[i][k];
+          dc[k] = on[i] ? d * rest[i][k] : 0.0f;
+          dz[k] = on[i] ? d * (hp[i][k] - c[i][k]) * (a[i][k] * rest[i][k]) : 0.0f;
+          start[k] = a[i][k] * d;
+        }
+        if (p.dgates && at.there && u < u_end) {
+          store4_upto(out + t * p.dg_t, at.left, dz);
+          store4_upto(out + t * p.dg_t + p.H, at.left, dc);
+        }
+      }
+      if constexpr (S == 1) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) e[k] = start[k];
+      }
+    }
+  }
+
+  if (!at.there) return;
+  if constexpr (MAPS) {
+    if (strand == 0) {
+      float* m = p.maps + channel * 4 + static_cast<int64_t>(2 * split) * lanes4;
+      *reinterpret_cast<float4*>(m) = make_float4(prod[0], prod[1], prod[2], prod[3]);
+      *reinterpret_cast<float4*>(m + lanes4) = make_float4(e[0], e[1], e[2], e[3]);
+    }
+  } else if (p.dh0 && split == p.splits - 1 && strand == 0) {
+    store4_upto(p.dh0 + at.n * p.H + at.c, at.left, e);
+  }
+}
+
+// How a problem is laid out; the same for both directions but for the steps of a tile.
+struct Plan {
+  bool walk;     // a thread walks the steps
+  int splits;
+  int64_t per_split;
+};
+Plan plan_for(int64_t T, int64_t N, int64_t H, int steps) {
+  const int64_t lanes = N * ((H + 3) / 4);
+  if (lanes >= kManyLanes || T <= kFewSteps) return {true, 1, T};
+  const int64_t tile = static_cast<int64_t>(kStrands) * steps;
+  const int64_t tiles = (T + tile - 1) / tile;
+  const int64_t groups = (lanes + kLanes - 1) / kLanes;
+  int64_t splits = kTargetGroups / groups;
+  splits = splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits;
+  splits = splits < tiles ? splits : tiles;
+  const int64_t per = (tiles + splits - 1) / splits * tile;
+  return {false, static_cast<int>((T + per - 1) / per), per};
+}
+size_t maps_bytes(int64_t T, int64_t N, int64_t H, int steps) {
+  const Plan q = plan_for(T, N, H, steps);
+  return q.splits > 1 ? static_cast<size_t>(q.splits) * 2 * N * ((H + 3) / 4) * 4 * sizeof(float) : 0;
+}
+
+template <typename T>
+void launch_fwd(ScanArgs a, const Plan& q, hipStream_t st) {
+  const int64_t lanes = a.N * a.Hq;
+  if (q.walk) {
+    scan_fwd_kernel<T, kThreads, 1, false><<<(lanes + kThreads - 1) / kThreads, kThreads, 0, st>>>(a);
+    return;
+  }
+  const unsigned groups = static_cast<unsigned>((lanes + kLanes - 1) / kLanes);
+  if (q.splits > 1)  // the last split's map starts nothing
+    scan_fwd_kernel<T, kLanes, kStrands, true><<<dim3(groups, q.splits - 1), kThreads, 0, st>>>(a);
+  scan_fwd_kernel<T, kLanes, kStrands, false><<<dim3(groups, q.splits), kThreads, 0, st>>>(a);
+}
+template <typename T>
+void launch_bwd(ScanArgs a, const Plan& q, hipStream_t st) {
+  const int64_t lanes = a.N * a.Hq;
+  if (q.walk) {
+    scan_bwd_kernel<T, kThreads, 1, false><<<(lanes + kThreads - 1) / kThreads, kThreads, 0, st>>>(a);
+    return;
+  }
+  const unsigned groups = static_cast<unsigned>((lanes + kLanes - 1) / kLanes);
+  if (q.splits > 1)
+    scan_bwd_kernel<T, kLanes, kStrands, true><<<dim3(groups, q.splits - 1), kThreads, 0, st>>>(a);
+  scan_bwd_kernel<T, kLanes, kStrands, false><<<dim3(groups, q.splits), kThreads, 0, st>>>(a);
+}
+
+int check_sizes(const char* what, int dtype, int64_t T, int64_t N, int64_t H) {
+  SPMI_REQUIRE(dtype == SPMI_DTYPE_F32 || dtype == SPMI_DTYPE_BF16, SPMI_ERR_INVALID_ARG, "%s: dtype %d", what, dtype);
+  SPMI_REQUIRE(T >= 0 && N >= 0 && H >= 1, SPMI_ERR_INVALID_ARG, "%s: T=%lld N=%lld H=%lld", what, (long long)T,
+               (long long)N, (long long)H);
+  // blockIdx.x counts workgroups of at least 32 lanes of four units
+  SPMI_REQUIRE(H <= (1 << 24) && N <= (1ll << 36) / H, SPMI_ERR_UNSUPPORTED, "%s: N=%lld H=%lld is too large", what,
+               (long long)N, (long long)H);
+  return SPMI_OK;
+}
+
+// ---- the single step on the node memory ------------------------------------------------------
+
+struct StepArgs {
+  const void* gates;
+  int64_t ldg;
+  float* mem;          // [nodes, H]
+  const int64_t* ids;  // nullable: row i of the gates belongs to node i
+  int64_t M, nodes;
+  int H, Hq;
+  float* out;          // [M, H]
+  float* before;       // nullable, [M, H]: the rows' old states
+  bool write;          // ids == nullptr only: the new states go to the memory as well
+  int32_t* owner;      // nullable, [nodes]: the entries of the named nodes are cleared
+};
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void step_kernel(StepArgs p) {
+  const int64_t total = p.M * p.Hq;
+  for (int64_t j = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; j < total;
+       j += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int64_t row = j / p.Hq;
+    const int c = static_cast<int>(j - row * p.Hq) * 4, left = p.H - c;
+    const int64_t node = p.ids ? p.ids[row] : row;
+    float z[4], cand[4], h[4];
+    const T* gates = static_cast<const T*>(p.gates) + row * p.ldg + c;
+    load4_upto(gates, left, 0.0f, z);
+    load4_upto(gates + p.H, left, 0.0f, cand);
+    const bool known = node >= 0 && node < p.nodes;
+    if (known) {
+      load4_upto(p.mem + node * p.H + c, left, 0.0f, h);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) h[k] = __builtin_nanf("");
+    }
+    if (p.before) store4_upto(p.before + row * p.H + c, left, h);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float a, rest;
+      gate_pair(z[k], a, rest);
+      h[k] = __builtin_fmaf(a, h[k], rest * cand[k]);
+    }
+    store4_upto(p.out + row * p.H + c, left, h);
+    if (p.write && known) store4_upto(p.mem + node * p.H + c, left, h);
+    if (p.owner && known && c == 0) p.owner[node] = -1;
+  }
+}
+
+// The last of the rows that name a node.
+__global__ void step_owner_kernel(const int64_t* ids, int64_t M, int64_t nodes, int32_t* owner) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (i < M && ids[i] >= 0 && ids[i] < nodes) atomicMax(&owner[ids[i]], static_cast<int32_t>(i));
+}
+
+// New states to the memory: a row is copied if no later row names its node.  `owner` holds the
+// last row of each named node, or is null and the wave looks through the later ids itself.
+__global__ __launch_bounds__(kThreads) void step_write_kernel(StepArgs p) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t row = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 6; row < p.M;
+       row += (static_cast<int64_t>(gridDim.x) * kThreads) >> 6) {
+    const int64_t node = p.ids[row];
+    if (node < 0 || node >= p.nodes) continue;
+    bool last = true;
+    if (p.owner) {
+      last = p.owner[node] == row;
+    } else {
+      for (int64_t i = row + 1 + lane; i < p.M; i += 64) last = last && p.ids[i] != node;
+      last = __all(last);
+    }
+    if (!last) continue;
+    for (int c = lane * 4; c < p.H; c += 256) {
+      float h[4];
+      load4_upto(p.out + row * p.H + c, p.H - c, 0.0f, h);
+      store4_upto(p.mem + node * p.H + c, p.H - c, h);
+    }
+  }
+}
+
+// Up to this many rows the ids behind a row are looked through (one launch less, no workspace).
+constexpr int64_t kLookRows = 1024;
+
+}  // namespace
+
+extern "C" {
+
+size_t spmi_gated_scan_fwd_workspace_bytes(int64_t T, int64_t N, int64_t H) {
+  return T > 0 && N > 0 && H > 0 ? maps_bytes(T, N, H, kFwdSteps) : 0;
+}
+size_t spmi_gated_scan_bwd_workspace_bytes(int64_t T, int64_t N, int64_t H) {
+  return T > 0 && N > 0 && H > 0 ? maps_bytes(T, N, H, kBwdSteps) : 0;
+}
+
+int spmi_gated_scan_fwd(const void* gates, int dtype, int64_t gates_t, int64_t gates_n, const float* h0, int64_t h0_n,
+                        const uint8_t* active, int64_t active_t, int64_t active_n, int64_t T, int64_t N, int64_t H,
+                        void* h, int64_t h_t, int64_t h_n, float* last, void* ws, size_t ws_bytes, void* stream) {
+  if (int rc = check_sizes("spmi_gated_scan_fwd", dtype, T, N, H)) return rc;
+  if (N == 0) return SPMI_OK;
+  SPMI_REQUIRE(last && (T == 0 || (gates && h)), SPMI_ERR_INVALID_ARG, "spmi_gated_scan_fwd: null pointer");
+  const Plan q = plan_for(T, N, H, kFwdSteps);
+  SPMI_REQUIRE(q.splits == 1 || (ws && ws_bytes >= maps_bytes(T, N, H, kFwdSteps)), SPMI_ERR_WORKSPACE,
+               "spmi_gated_scan_fwd: workspace of %zu bytes is too small", ws_bytes);
+  SPMI_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 15) == 0, SPMI_ERR_INVALID_ARG,
+               "spmi_gated_scan_fwd: the workspace must be aligned to 16 bytes");
+  ScanArgs a{};
+  a.gates = gates; a.gates_t = gates_t; a.gates_n = gates_n;
+  a.h0 = h0; a.h0_n = h0_n;
+  a.active = active; a.active_t = active_t; a.active_n = active_n;
+  a.h = h; a.h_t = h_t; a.h_n = h_n; a.last = last;
+  a.T = T; a.N = N; a.H = static_cast<int>(H); a.Hq = static_cast<int>((H + 3) / 4);
+  a.per_split = q.per_split; a.splits = q.splits; a.maps = static_cast<float*>(ws);
+  if (dtype == SPMI_DTYPE_F32) launch_fwd<float>(a, q, as_stream(stream));
+  else launch_fwd<bf16>(a, q, as_stream(stream));
+  SPMI_CHECK_LAUNCH("spmi_gated_scan_fwd");
+  return SPMI_OK;
+}
+
+int spmi_gated_scan_bwd(const void* gates, int dtype, int64_t gates_t, int64_t gates_n, const float* h0, int64_t h0_n,
+                        const uint8_t* active, int64_t active_t, int64_t active_n, int64_t T, int64_t N, int64_t H,
+                        const void* h, int64_t h_t, int64_t h_n, const void* g, int64_t g_t, int64_t g_n,
+                        const float* g_last, int64_t gl_n, void* dgates, int64_t dg_t, int64_t dg_n, float* dh0,
+                        void* ws, size_t ws_bytes, void* stream) {
+  if (int rc = check_sizes("spmi_gated_scan_bwd", dtype, T, N, H)) return rc;
+  if (N == 0 || (T == 0 && !dh0)) return SPMI_OK;
+  SPMI_REQUIRE((T == 0 || gates) && (T <= 1 || h), SPMI_ERR_INVALID_ARG, "spmi_gated_scan_bwd: null pointer");
+  const Plan q = plan_for(T, N, H, kBwdSteps);
+  SPMI_REQUIRE(q.splits == 1 || (ws && ws_bytes >= maps_bytes(T, N, H, kBwdSteps)), SPMI_ERR_WORKSPACE,
+               "spmi_gated_scan_bwd: workspace of %zu bytes is too small", ws_bytes);
+  SPMI_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 15) == 0, SPMI_ERR_INVALID_ARG,
+               "spmi_gated_scan_bwd: the workspace must be aligned to 16 bytes");
+  ScanArgs a{};
+  a.gates = gates; a.gates_t = gates_t; a.gates_n = gates_n;
+  a.h0 = h0; a.h0_n = h0_n;
+  a.active = active; a.active_t = active_t; a.active_n = active_n;
+  a.h = const_cast<void*>(h); a.h_t = h_t; a.h_n = h_n;
+  a.g = g; a.g_t = g_t; a.g_n = g_n; a.g_last = g_last; a.gl_n = gl_n;
+  a.dgates = dgates; a.dg_t = dg_t; a.dg_n = dg_n; a.dh0 = dh0;
+  a.T = T; a.N = N; a.H = static_cast<int>(H); a.Hq = static_cast<int>((H + 3) / 4);
+  a.per_split = q.per_split; a.splits = q.splits; a.maps = static_cast<float*>(ws);
+  if (dtype == SPMI_DTYPE_F32) launch_bwd<float>(a, q, as_stream(stream));
+  else launch_bwd<bf16>(a, q, as_stream(stream));
+  SPMI_CHECK_LAUNCH("spmi_gated_scan_bwd");
+  return SPMI_OK;
+}
+
+size_t spmi_gated_step_workspace_bytes(int64_t M, int64_t nodes) {
+  return M > kLookRows && nodes > 0 ? static_cast<size_t>(nodes) * sizeof(int32_t) : 0;
+}
+
+int spmi_gated_step(const void* gates, int dtype, int64_t ldg, float* h_mem, int64_t nodes, const int64_t* ids,
+                    int64_t M, int64_t H, float* h_out, float* h_before, int mem_write, void* ws, size_t ws_bytes,
+                    void* stream) {
+  if (int rc = check_sizes("spmi_gated_step", dtype, 1, M, H)) return rc;
+  SPMI_REQUIRE(nodes >= 0 && M < (1ll << 31), SPMI_ERR_INVALID_ARG, "spmi_gated_step: %lld nodes, %lld rows",
+               (long long)nodes, (long long)M);
+  SPMI_REQUIRE(ids || M <= nodes, SPMI_ERR_INVALID_ARG, "spmi_gated_step: more rows than nodes");
+  if (M == 0) return SPMI_OK;
+  SPMI_REQUIRE(gates && h_out && (h_mem || nodes == 0), SPMI_ERR_INVALID_ARG, "spmi_gated_step: null pointer");
+  const bool scatter = ids && mem_write;
+  const bool owners = scatter && M > kLookRows;
+  SPMI_REQUIRE(!owners || (ws && ws_bytes >= spmi_gated_step_workspace_bytes(M, nodes)) || nodes == 0,
+               SPMI_ERR_WORKSPACE, "spmi_gated_step: workspace of %zu bytes is too small", ws_bytes);
+  hipStream_t st = as_stream(stream);
+  StepArgs a{gates, ldg, h_mem, ids, M, nodes, static_cast<int>(H), static_cast<int>((H + 3) / 4), h_out, h_before,
+             mem_write != 0 && !ids, owners ? static_cast<int32_t*>(ws) : nullptr};
+  const int64_t need = (M * a.Hq + kThreads - 1) / kThreads;
+  const unsigned grid = static_cast<unsigned>(need < 8192 ? need : 8192);
+  if (dtype == SPMI_DTYPE_F32) step_kernel<float><<<grid, kThreads, 0, st>>>(a);
+  else step_kernel<bf16><<<grid, kThreads, 0, st>>>(a);
+  SPMI_CHECK_LAUNCH("spmi_gated_step");
+  if (scatter && nodes > 0) {
+    if (owners) {
+      step_owner_kernel<<<static_cast<unsigned>((M + 255) / 256), 256, 0, st>>>(ids, M, nodes, a.owner);
+      SPMI_CHECK_LAUNCH("spmi_gated_step");
+    }
+    const int64_t blocks = (M + 3) / 4;
+    step_write_kernel<<<static_cast<unsigned>(blocks < 8192 ? blocks : 8192), kThreads, 0, st>>>(a);
+    SPMI_CHECK_LAUNCH("spmi_gated_step");
+  }
+  return SPMI_OK;
+}
+
+}  // extern "C"

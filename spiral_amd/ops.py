@@ -14,6 +14,8 @@ from typing import Optional, Tuple
 import torch
 
 from . import _native as nv
+from .block_ops import (  # noqa: F401
+    INT8_MAX_INNER, LAYER_NORM_MAX_WIDTH, gated_scan, gated_step, layer_norm, linear_int8, quantize_rows_int8)
 from .graph import _ACT_CODES, aggregate
 
 
