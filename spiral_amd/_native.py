@@ -188,8 +188,17 @@ def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+def current_device() -> int:
+    return torch._C._cuda_getDevice()
+
+
+def raw_stream(device: int) -> int:
+    """The current stream of a device as an address, without building a torch.cuda.Stream."""
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
 def stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    return raw_stream(current_device())
 
 
 def require_cuda(*tensors: Optional[torch.Tensor]) -> None:

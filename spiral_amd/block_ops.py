@@ -4,7 +4,11 @@ part of `spiral_amd.ops`, which offers them under the same names.
 
 Each call queues its kernels on torch's current stream of the device its tensors live on, takes its
 workspace from torch's allocator for that stream, and waits for nothing, so it can be captured into
-a graph and run on any stream."""
+a graph and run on any stream.  (torch's own rule holds for capturing a backward pass: no eager graph
+of the same leaves may be alive on another stream meanwhile.)
+
+A small call is bound by the host: a launch costs ~3 us there and torch.empty ~1 us, so the wrappers
+look at each argument once, ask for the raw stream, and switch the device only where it differs."""
 from __future__ import annotations
 
 from typing import Optional, Tuple
@@ -15,21 +19,37 @@ from torch.autograd.function import once_differentiable
 from . import _native as nv
 from .graph import _ACT_CODES
 
+_F32 = torch.float32
 _DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1}
+LAYER_NORM_MAX_WIDTH = 16384  # spmi_layer_norm_max_width()
+INT8_MAX_INNER = 131072       # 127^2 times this still fits the 32-bit sums
+
+_tracking = torch.is_grad_enabled
+_empty = torch.empty
 
 
-def _rows_dtype(t: torch.Tensor, what: str) -> int:
+def _refuse(what: str) -> None:
+    raise nv.SpmiError(what)
+
+
+def _code(t: torch.Tensor, what: str) -> int:
     code = _DTYPE_CODES.get(t.dtype)
     if code is None:
-        raise nv.SpmiError(f"{what} must be float32 or bfloat16, got {t.dtype}")
+        _refuse(f"{what} must be float32 or bfloat16, got {t.dtype}")
     return code
 
 
-def _same_device(t: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
-    nv.require_cuda(t, *others)
+def _device_of(t: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """The device all of these live on."""
+    at = t.get_device()
     for o in others:
-        if o is not None and o.device != t.device:
-            raise nv.SpmiError(f"tensors on different devices: {t.device} and {o.device}")
+        if o is not None and o.get_device() != at:
+            at = -1
+            break
+    if at < 0:
+        nv.require_cuda(t, *others)
+        _refuse(f"tensors on different devices: {[str(o.device) for o in (t, *others) if o is not None]}")
+    return at
 
 
 def _rows_of(t: torch.Tensor) -> torch.Tensor:
@@ -39,63 +59,97 @@ def _rows_of(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
-def _workspace(nbytes: int, device: torch.device) -> Optional[torch.Tensor]:
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-
-
-def _tracked(*tensors: Optional[torch.Tensor]) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-# --------------------------------------------------------------------------- layer norm
-LAYER_NORM_MAX_WIDTH = 16384  # spmi_layer_norm_max_width()
+def _units_last(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def _float_vector(v: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return None if v is None else v.detach().to(torch.float32).contiguous()
+    """A vector of parameters as the kernels read it: float32, contiguous."""
+    if v is None or (v.dtype == _F32 and v.is_contiguous()):
+        return v
+    return v.detach().to(_F32).contiguous()
 
 
-def _layer_norm_fwd(x, weight, bias, eps, keep):
-    xd = _rows_of(x.detach())
-    m, d = xd.shape
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _workspace(nbytes: int, device: torch.device) -> Optional[torch.Tensor]:
+    return _empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _launch(name: str, at: int, *args) -> None:
+    """Queue entry point `name` on the current stream of device `at`."""
+    fn = getattr(nv.lib(), name)
+    if nv.current_device() == at:
+        rc = fn(*args, nv.raw_stream(at))
+    else:
+        with torch.cuda.device(at):
+            rc = fn(*args, nv.raw_stream(at))
+    if rc:
+        nv.check(rc, name)
+
+
+class _Operator(torch.autograd.Function):
+    """Base of the operators below: `gradients(ctx, *g)` is the backward pass.  It runs kernels
+    autograd does not see, so a second derivative through it raises instead of being wrong; the
+    wrapper for that (a few us) is only taken where a graph of the backward pass is recorded."""
+
+    @staticmethod
+    def gradients(ctx, *g):
+        raise NotImplementedError
+
+    @classmethod
+    def _bind(cls):
+        plain, once = cls.gradients, once_differentiable(cls.gradients)
+        cls.backward = staticmethod(lambda ctx, *g: once(ctx, *g) if _tracking() else plain(ctx, *g))
+        return cls
+
+
+# --------------------------------------------------------------------------- layer norm
+def _layer_norm_fwd(x, weight, bias, eps, code, at, keep):
+    xr = _rows_of(x)
+    m, d = xr.shape
     w, b = _float_vector(weight), _float_vector(bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty(m, 2, dtype=torch.float32, device=x.device) if keep else None
-    with torch.cuda.device(x.device):
-        nv.check(nv.lib().spmi_layer_norm_fwd(nv.ptr(xd), _DTYPE_CODES[x.dtype], xd.stride(0), m, d, nv.ptr(w),
-                                              nv.ptr(b), eps, nv.ptr(y), d, nv.ptr(stats), nv.stream()),
-                 "spmi_layer_norm_fwd")
+    y = _empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = _empty(m, 2, dtype=_F32, device=x.device) if keep else None
+    _launch("spmi_layer_norm_fwd", at, xr.data_ptr(), code, xr.stride(0), m, d, _ptr(w), _ptr(b), eps, y.data_ptr(),
+            d, _ptr(stats))
     return y, stats
 
 
-class _LayerNorm(torch.autograd.Function):
+class _LayerNorm(_Operator):
     @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, stats = _layer_norm_fwd(x, weight, bias, eps, True)
+    def forward(ctx, x, weight, bias, eps, code, at):
+        y, stats = _layer_norm_fwd(x, weight, bias, eps, code, at, True)
         ctx.save_for_backward(x, weight, stats)
-        ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.plain = (code, at, None if bias is None else bias.dtype)
         return y
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
+    def gradients(ctx, g):
         x, weight, stats = ctx.saved_tensors
+        code, at, bias_dtype = ctx.plain
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        xd, gd = _rows_of(x.detach()), _rows_of(g)
-        m, d = xd.shape
+        xr, gr = _rows_of(x), _rows_of(g)
+        m, d = xr.shape
         dev = x.device
         w = _float_vector(weight)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-        dw = torch.empty(d, dtype=torch.float32, device=dev) if need_w else None
-        db = torch.empty(d, dtype=torch.float32, device=dev) if need_b else None
-        lib = nv.lib()
-        ws_bytes = lib.spmi_layer_norm_bwd_workspace_bytes(m, d) if need_w or need_b else 0
-        with torch.cuda.device(dev):
-            ws = _workspace(ws_bytes, dev)
-            nv.check(lib.spmi_layer_norm_bwd(nv.ptr(xd), nv.ptr(gd), _DTYPE_CODES[x.dtype], xd.stride(0),
-                                             gd.stride(0), m, d, nv.ptr(w), nv.ptr(stats), nv.ptr(dx), d, nv.ptr(dw),
-                                             nv.ptr(db), nv.ptr(ws), ws_bytes, nv.stream()), "spmi_layer_norm_bwd")
-        return (dx, dw.to(weight.dtype) if need_w else None, db.to(ctx.bias_dtype) if need_b else None, None)
+        dx = _empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+        dw = _empty(d, dtype=_F32, device=dev) if need_w else None
+        db = _empty(d, dtype=_F32, device=dev) if need_b else None
+        ws_bytes = nv.lib().spmi_layer_norm_bwd_workspace_bytes(m, d) if need_w or need_b else 0
+        ws = _workspace(ws_bytes, dev)
+        _launch("spmi_layer_norm_bwd", at, xr.data_ptr(), gr.data_ptr(), code, xr.stride(0), gr.stride(0), m, d,
+                _ptr(w), stats.data_ptr(), _ptr(dx), d, _ptr(dw), _ptr(db), _ptr(ws), ws_bytes)
+        if need_w and weight.dtype != _F32:
+            dw = dw.to(weight.dtype)
+        if need_b and bias_dtype != _F32:
+            db = db.to(bias_dtype)
+        return dx, dw, db, None, None, None
+
+
+_LayerNorm._bind()
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -104,92 +158,90 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     differentiable in x, weight and bias.  x: float32 or bfloat16 of any strides, D from 1 to 16384;
     weight and bias: [D] in either type, or None.  Statistics and gradient sums are float32; the
     gradients of weight and bias are added up in a fixed order (the same bits every time)."""
-    _rows_dtype(x, "layer_norm: x")
+    code = _code(x, "layer_norm: x")
     if x.dim() < 1 or not 1 <= x.shape[-1] <= LAYER_NORM_MAX_WIDTH:
-        raise nv.SpmiError(f"layer_norm: the last dimension of x must be 1 to {LAYER_NORM_MAX_WIDTH}, got "
-                           f"{tuple(x.shape)}")
-    for name, v in (("weight", weight), ("bias", bias)):
+        _refuse(f"layer_norm: the last dimension of x must be 1 to {LAYER_NORM_MAX_WIDTH}, got {tuple(x.shape)}")
+    grad = x.requires_grad
+    for v in (weight, bias):
         if v is not None:
-            _rows_dtype(v, f"layer_norm: {name}")
+            _code(v, "layer_norm: weight and bias")
             if v.shape != x.shape[-1:]:
-                raise nv.SpmiError(f"layer_norm: {name} must have shape ({x.shape[-1]},), got {tuple(v.shape)}")
+                _refuse(f"layer_norm: weight and bias must have shape ({x.shape[-1]},), got {tuple(v.shape)}")
+            grad = grad or v.requires_grad
     eps = float(eps)
     if not 0.0 <= eps < float("inf"):
-        raise nv.SpmiError(f"layer_norm: eps must be finite and not negative, got {eps}")
-    _same_device(x, weight, bias)
-    if _tracked(x, weight, bias):
-        return _LayerNorm.apply(x, weight, bias, eps)
-    return _layer_norm_fwd(x, weight, bias, eps, False)[0]
+        _refuse(f"layer_norm: eps must be finite and not negative, got {eps}")
+    at = _device_of(x, weight, bias)
+    if grad and _tracking():
+        return _LayerNorm.apply(x, weight, bias, eps, code, at)
+    return _layer_norm_fwd(x, weight, bias, eps, code, at, False)[0]
 
 
 # --------------------------------------------------------------------------- gated linear recurrence
-def _units_last(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
-def _step_strides(t: torch.Tensor, batch_first: bool) -> Tuple[int, int]:
+def _step_strides(t: Optional[torch.Tensor], batch_first: bool) -> Tuple[int, int]:
     """Strides along steps and along nodes."""
+    if t is None:
+        return 0, 0
     return (t.stride(1), t.stride(0)) if batch_first else (t.stride(0), t.stride(1))
 
 
-def _scan_call(direction, gates, h0, active, batch_first, h, last, g=None, g_last=None, dgates=None, dh0=None):
+def _scan_head(gates, h0, active, batch_first, code, h):
+    """The arguments both directions begin with."""
+    n, t = gates.shape[:2] if batch_first else (gates.shape[1], gates.shape[0])
+    return (gates.data_ptr(), code, *_step_strides(gates, batch_first), _ptr(h0), 0 if h0 is None else h0.stride(0),
+            _ptr(active), *_step_strides(active, batch_first), t, n, gates.shape[2] // 2, h.data_ptr(),
+            *_step_strides(h, batch_first))
+
+
+def _scan_bwd(gates, h0, active, batch_first, code, at, h, g, g_last, dgates, dh0):
+    head = _scan_head(gates, h0, active, batch_first, code, h)
+    ws_bytes = nv.lib().spmi_gated_scan_bwd_workspace_bytes(*head[9:12])
+    ws = _workspace(ws_bytes, gates.device)
+    _launch("spmi_gated_scan_bwd", at, *head, _ptr(g), *_step_strides(g, batch_first), _ptr(g_last),
+            0 if g_last is None else g_last.stride(0), _ptr(dgates), *_step_strides(dgates, batch_first), _ptr(dh0),
+            _ptr(ws), ws_bytes)
+
+
+def _scan_fwd(gates, h0, active, batch_first, code, at):
+    gates = _units_last(gates)
     n, t = gates.shape[:2] if batch_first else (gates.shape[1], gates.shape[0])
     hd = gates.shape[2] // 2
-    lib = nv.lib()
-    a_t, a_n = (0, 0) if active is None else _step_strides(active, batch_first)
-    head = (nv.ptr(gates), _DTYPE_CODES[gates.dtype], *_step_strides(gates, batch_first), nv.ptr(h0),
-            0 if h0 is None else h0.stride(0), nv.ptr(active), a_t, a_n, t, n, hd, nv.ptr(h),
-            *_step_strides(h, batch_first))
-    with torch.cuda.device(gates.device):
-        if direction == "fwd":
-            ws_bytes = lib.spmi_gated_scan_fwd_workspace_bytes(t, n, hd)
-            ws = _workspace(ws_bytes, gates.device)
-            nv.check(lib.spmi_gated_scan_fwd(*head, nv.ptr(last), nv.ptr(ws), ws_bytes, nv.stream()),
-                     "spmi_gated_scan_fwd")
-        else:
-            ws_bytes = lib.spmi_gated_scan_bwd_workspace_bytes(t, n, hd)
-            ws = _workspace(ws_bytes, gates.device)
-            g_t, g_n = (0, 0) if g is None else _step_strides(g, batch_first)
-            d_t, d_n = (0, 0) if dgates is None else _step_strides(dgates, batch_first)
-            nv.check(lib.spmi_gated_scan_bwd(*head, nv.ptr(g), g_t, g_n, nv.ptr(g_last),
-                                             0 if g_last is None else g_last.stride(0), nv.ptr(dgates), d_t, d_n,
-                                             nv.ptr(dh0), nv.ptr(ws), ws_bytes, nv.stream()), "spmi_gated_scan_bwd")
-
-
-def _scan_fwd(gates, h0, active, batch_first):
-    gd = _units_last(gates.detach())
-    hd = gd.shape[2] // 2
-    h0d = None if h0 is None else _units_last(h0.detach())
-    h = torch.empty(*gd.shape[:2], hd, dtype=gd.dtype, device=gd.device)
-    last = torch.empty(gd.shape[0 if batch_first else 1], hd, dtype=torch.float32, device=gd.device)
-    _scan_call("fwd", gd, h0d, active, batch_first, h, last)
+    if h0 is not None:
+        h0 = _units_last(h0)
+    h = _empty(*gates.shape[:2], hd, dtype=gates.dtype, device=gates.device)
+    last = _empty(n, hd, dtype=_F32, device=gates.device)
+    ws_bytes = nv.lib().spmi_gated_scan_fwd_workspace_bytes(t, n, hd)
+    ws = _workspace(ws_bytes, gates.device)
+    _launch("spmi_gated_scan_fwd", at, *_scan_head(gates, h0, active, batch_first, code, h), last.data_ptr(),
+            _ptr(ws), ws_bytes)
     return h, last
 
 
-class _GatedScan(torch.autograd.Function):
+class _GatedScan(_Operator):
     @staticmethod
-    def forward(ctx, gates, h0, active, batch_first):
-        h, last = _scan_fwd(gates, h0, active, batch_first)
+    def forward(ctx, gates, h0, active, batch_first, code, at):
+        h, last = _scan_fwd(gates, h0, active, batch_first, code, at)
         ctx.save_for_backward(gates, h0, active, h)
-        ctx.batch_first = batch_first
+        ctx.plain = (batch_first, code, at)
         ctx.set_materialize_grads(False)
         return h, last
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, g, g_last):
+    def gradients(ctx, g, g_last):
         gates, h0, active, h = ctx.saved_tensors
+        batch_first, code, at = ctx.plain
         need_gates, need_h0 = ctx.needs_input_grad[:2]
         if g is None and g_last is None:
-            return None, None, None, None
-        gd = _units_last(gates.detach())
-        h0d = None if h0 is None else _units_last(h0.detach())
-        dgates = torch.empty(gd.shape, dtype=gd.dtype, device=gd.device) if need_gates else None
-        dh0 = torch.empty(h0.shape, dtype=torch.float32, device=gd.device) if need_h0 else None
-        _scan_call("bwd", gd, h0d, active, ctx.batch_first, h, None,
-                   None if g is None else _units_last(g), None if g_last is None else _units_last(g_last),
-                   dgates, dh0)
-        return dgates, dh0, None, None
+            return None, None, None, None, None, None
+        gates = _units_last(gates)
+        dgates = _empty(gates.shape, dtype=gates.dtype, device=gates.device) if need_gates else None
+        dh0 = _empty(h0.shape, dtype=_F32, device=gates.device) if need_h0 else None
+        _scan_bwd(gates, None if h0 is None else _units_last(h0), active, batch_first, code, at, h,
+                  None if g is None else _units_last(g), None if g_last is None else _units_last(g_last), dgates, dh0)
+        return dgates, dh0, None, None, None, None
+
+
+_GatedScan._bind()
 
 
 def gated_scan(gates: torch.Tensor, h0: Optional[torch.Tensor] = None, active: Optional[torch.Tensor] = None,
@@ -204,59 +256,58 @@ def gated_scan(gates: torch.Tensor, h0: Optional[torch.Tensor] = None, active: O
     are not used (they may hold anything) and receive a zero gradient.  A node that joins late or a
     sequence that ends early is described by it.  Returns the states [T, N, H] ([N, T, H]) in the
     type of `gates` and the last state [N, H] in float32 (h0 where no step is active)."""
-    _rows_dtype(gates, "gated_scan: gates")
+    code = _code(gates, "gated_scan: gates")
     if gates.dim() != 3 or gates.shape[2] < 2 or gates.shape[2] % 2:
-        raise nv.SpmiError(f"gated_scan: gates must be [T, N, 2H], got {tuple(gates.shape)}")
+        _refuse(f"gated_scan: gates must be [T, N, 2H], got {tuple(gates.shape)}")
+    batch_first = bool(batch_first)
     n, hd = gates.shape[0 if batch_first else 1], gates.shape[2] // 2
-    if h0 is not None and (h0.shape != (n, hd) or h0.dtype != torch.float32):
-        raise nv.SpmiError(f"gated_scan: h0 must be float32 [{n}, {hd}], got {h0.dtype} {tuple(h0.shape)}")
-    if active is not None:
-        if active.dtype != torch.bool or active.shape != gates.shape[:2]:
-            raise nv.SpmiError(f"gated_scan: active must be bool {tuple(gates.shape[:2])}, got {active.dtype} "
-                               f"{tuple(active.shape)}")
-    _same_device(gates, h0, active)
-    if _tracked(gates, h0):
-        return _GatedScan.apply(gates, h0, active, bool(batch_first))
-    return _scan_fwd(gates, h0, active, bool(batch_first))
+    grad = gates.requires_grad
+    if h0 is not None:
+        if h0.shape != (n, hd) or h0.dtype != _F32:
+            _refuse(f"gated_scan: h0 must be float32 [{n}, {hd}], got {h0.dtype} {tuple(h0.shape)}")
+        grad = grad or h0.requires_grad
+    if active is not None and (active.dtype != torch.bool or active.shape != gates.shape[:2]):
+        _refuse(f"gated_scan: active must be bool {tuple(gates.shape[:2])}, got {active.dtype} {tuple(active.shape)}")
+    at = _device_of(gates, h0, active)
+    if grad and _tracking():
+        return _GatedScan.apply(gates, h0, active, batch_first, code, at)
+    return _scan_fwd(gates, h0, active, batch_first, code, at)
 
 
-def _step_fwd(gates, h_mem, ids, mem_write, keep):
-    gd = gates.detach()
-    gd = gd if gd.stride(1) == 1 else gd.contiguous()
-    m, hd = gd.shape[0], gd.shape[1] // 2
-    dev = gd.device
-    h = torch.empty(m, hd, dtype=torch.float32, device=dev)
-    before = torch.empty(m, hd, dtype=torch.float32, device=dev) if keep else None
-    lib = nv.lib()
+def _step_fwd(gates, h_mem, ids, mem_write, code, at, keep):
+    gates = _units_last(gates)
+    m, hd = gates.shape[0], gates.shape[1] // 2
     nodes = h_mem.shape[0]
-    ws_bytes = lib.spmi_gated_step_workspace_bytes(m, nodes) if mem_write and ids is not None else 0
-    with torch.cuda.device(dev):
-        ws = _workspace(ws_bytes, dev)
-        nv.check(lib.spmi_gated_step(nv.ptr(gd), _DTYPE_CODES[gd.dtype], gd.stride(0), nv.ptr(h_mem), nodes,
-                                     nv.ptr(ids), m, hd, nv.ptr(h), nv.ptr(before), int(mem_write), nv.ptr(ws),
-                                     ws_bytes, nv.stream()), "spmi_gated_step")
+    h = _empty(m, hd, dtype=_F32, device=gates.device)
+    before = _empty(m, hd, dtype=_F32, device=gates.device) if keep else None
+    ws_bytes = nv.lib().spmi_gated_step_workspace_bytes(m, nodes) if mem_write and ids is not None else 0
+    ws = _workspace(ws_bytes, gates.device)
+    _launch("spmi_gated_step", at, gates.data_ptr(), code, gates.stride(0), h_mem.data_ptr(), nodes, _ptr(ids), m, hd,
+            h.data_ptr(), _ptr(before), mem_write, _ptr(ws), ws_bytes)
     if mem_write:
         torch.autograd.graph.increment_version(h_mem)
     return h, before
 
 
-class _GatedStep(torch.autograd.Function):
+class _GatedStep(_Operator):
     @staticmethod
-    def forward(ctx, gates, h_mem, ids, mem_write):
-        h, before = _step_fwd(gates, h_mem, ids, mem_write, True)
+    def forward(ctx, gates, h_mem, ids, mem_write, code, at):
+        h, before = _step_fwd(gates, h_mem, ids, mem_write, code, at, True)
         ctx.save_for_backward(gates, before)
+        ctx.plain = (code, at)
         return h
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        # the scan's backward over one step, with the rows' old states as its start
+    def gradients(ctx, g):
+        # the scan's backward pass over one step, with the rows' old states as its start
         gates, before = ctx.saved_tensors
-        gd = gates.detach()
-        gd = gd if gd.stride(1) == 1 else gd.contiguous()
-        dgates = torch.empty(gd.shape, dtype=gd.dtype, device=gd.device)
-        _scan_call("bwd", gd[None], before, None, False, before[None], None, None, _units_last(g), dgates[None])
-        return dgates, None, None, None
+        gates = _units_last(gates)
+        dgates = _empty(gates.shape, dtype=gates.dtype, device=gates.device)
+        _scan_bwd(gates[None], before, None, False, *ctx.plain, before[None], None, _units_last(g), dgates[None], None)
+        return dgates, None, None, None, None, None
+
+
+_GatedStep._bind()
 
 
 def gated_step(gates: torch.Tensor, h_mem: torch.Tensor, ids: Optional[torch.Tensor] = None,
@@ -270,50 +321,45 @@ def gated_step(gates: torch.Tensor, h_mem: torch.Tensor, ids: Optional[torch.Ten
     Every row starts from the memory as it was before the call.  Where `ids` names a node several
     times the memory keeps the last of its rows.  A row whose id is outside [0, nodes) comes out as
     NaN and is written nowhere else."""
-    _rows_dtype(gates, "gated_step: gates")
+    code = _code(gates, "gated_step: gates")
     if gates.dim() != 2 or gates.shape[1] < 2 or gates.shape[1] % 2:
-        raise nv.SpmiError(f"gated_step: gates must be [M, 2H], got {tuple(gates.shape)}")
+        _refuse(f"gated_step: gates must be [M, 2H], got {tuple(gates.shape)}")
     m, hd = gates.shape[0], gates.shape[1] // 2
-    if h_mem.dim() != 2 or h_mem.shape[1] != hd or h_mem.dtype != torch.float32 or not h_mem.is_contiguous():
-        raise nv.SpmiError(f"gated_step: the node memory must be contiguous float32 [nodes, {hd}], got "
-                           f"{h_mem.dtype} {tuple(h_mem.shape)}")
-    if h_mem.requires_grad and torch.is_grad_enabled():
-        raise nv.SpmiError("gated_step: the node memory is a state and takes no gradient")
+    if h_mem.dim() != 2 or h_mem.shape[1] != hd or h_mem.dtype != _F32 or not h_mem.is_contiguous():
+        _refuse(f"gated_step: the node memory must be contiguous float32 [nodes, {hd}], got {h_mem.dtype} "
+                f"{tuple(h_mem.shape)}")
+    if h_mem.requires_grad and _tracking():
+        _refuse("gated_step: the node memory is a state and takes no gradient")
     if ids is None:
         if m > h_mem.shape[0]:
-            raise nv.SpmiError("gated_step: more rows than nodes in the memory")
+            _refuse("gated_step: more rows than nodes in the memory")
     elif ids.dtype != torch.int64 or ids.shape != (m,):
-        raise nv.SpmiError(f"gated_step: ids must be int64 [{m}], got {ids.dtype} {tuple(ids.shape)}")
-    else:
+        _refuse(f"gated_step: ids must be int64 [{m}], got {ids.dtype} {tuple(ids.shape)}")
+    elif not ids.is_contiguous():
         ids = ids.contiguous()
-    _same_device(gates, h_mem, ids)
-    if _tracked(gates):
-        return _GatedStep.apply(gates, h_mem, ids, bool(mem_write))
-    return _step_fwd(gates, h_mem, ids, bool(mem_write), False)[0]
+    at = _device_of(gates, h_mem, ids)
+    mem_write = bool(mem_write)
+    if gates.requires_grad and _tracking():
+        return _GatedStep.apply(gates, h_mem, ids, mem_write, code, at)
+    return _step_fwd(gates, h_mem, ids, mem_write, code, at, False)[0]
 
 
 # --------------------------------------------------------------------------- 8-bit integers
-INT8_MAX_INNER = 131072  # 127^2 times this still fits the 32-bit sums
-
-
 def quantize_rows_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """Rows of x [..., K] (float32 or bfloat16) in 8-bit integers: `q` int8 of x's shape and `scale`
     float32 of its leading shape, x = q * scale to within half a scale.  With m the row's largest
     magnitude (at least 2^-120), scale = m / 127 and q = rint(x * (127 / m)), each operation rounded
     to float32.  A row with a value that is not finite gets q = 0 and scale = NaN.  Applied to a
     weight [N, K] this gives the arguments of `linear_int8`."""
-    code = _rows_dtype(x, "quantize_rows_int8: x")
+    code = _code(x, "quantize_rows_int8: x")
     if x.dim() < 1 or not 1 <= x.shape[-1] <= INT8_MAX_INNER:
-        raise nv.SpmiError(f"quantize_rows_int8: the last dimension of x must be 1 to {INT8_MAX_INNER}, got "
-                           f"{tuple(x.shape)}")
-    nv.require_cuda(x)
-    xd = _rows_of(x.detach())
-    m, k = xd.shape
-    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        nv.check(nv.lib().spmi_quantize_rows_i8(nv.ptr(xd), code, xd.stride(0), m, k, nv.ptr(q), k, nv.ptr(scale),
-                                                nv.stream()), "spmi_quantize_rows_i8")
+        _refuse(f"quantize_rows_int8: the last dimension of x must be 1 to {INT8_MAX_INNER}, got {tuple(x.shape)}")
+    at = _device_of(x)
+    xr = _rows_of(x)
+    m, k = xr.shape
+    q = _empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = _empty(x.shape[:-1], dtype=_F32, device=x.device)
+    _launch("spmi_quantize_rows_i8", at, xr.data_ptr(), code, xr.stride(0), m, k, q.data_ptr(), k, scale.data_ptr())
     return q, scale
 
 
@@ -326,37 +372,37 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     "leaky_relu" with `slope`) follow in float32, and the result [..., N] is rounded once to
     `out_dtype` (default: x's type).  weight: int8 [N, K], weight_scale: float32 [N]; K up to 131072.
     For serving: there is no backward pass, and a call that would need one is refused."""
-    code = _rows_dtype(x, "linear_int8: x")
+    code = _code(x, "linear_int8: x")
     if weight.dim() != 2 or weight.dtype != torch.int8:
-        raise nv.SpmiError(f"linear_int8: weight must be int8 [N, K], got {weight.dtype} {tuple(weight.shape)}")
+        _refuse(f"linear_int8: weight must be int8 [N, K], got {weight.dtype} {tuple(weight.shape)}")
     n, k = weight.shape
     if x.dim() < 1 or x.shape[-1] != k or not 1 <= k <= INT8_MAX_INNER:
-        raise nv.SpmiError(f"linear_int8: x {tuple(x.shape)} does not fit a weight {tuple(weight.shape)}")
-    if weight_scale.shape != (n,) or weight_scale.dtype != torch.float32:
-        raise nv.SpmiError(f"linear_int8: weight_scale must be float32 [{n}]")
+        _refuse(f"linear_int8: x {tuple(x.shape)} does not fit a weight {tuple(weight.shape)}")
+    if weight_scale.shape != (n,) or weight_scale.dtype != _F32:
+        _refuse(f"linear_int8: weight_scale must be float32 [{n}]")
+    grad = x.requires_grad or weight_scale.requires_grad
     if bias is not None:
         if bias.shape != (n,):
-            raise nv.SpmiError(f"linear_int8: bias must have shape ({n},), got {tuple(bias.shape)}")
-        _rows_dtype(bias, "linear_int8: bias")
-    if act not in _ACT_CODES:
-        raise nv.SpmiError(f"linear_int8: unknown activation {act!r}")
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    if out_dtype not in _DTYPE_CODES:
-        raise nv.SpmiError("linear_int8: out_dtype must be float32 or bfloat16")
-    if _tracked(x, weight_scale, bias):
-        raise nv.SpmiError("linear_int8 has no backward pass: call it under torch.no_grad()")
-    _same_device(x, weight, weight_scale, bias)
+            _refuse(f"linear_int8: bias must have shape ({n},), got {tuple(bias.shape)}")
+        _code(bias, "linear_int8: bias")
+        grad = grad or bias.requires_grad
+    act_code = _ACT_CODES.get(act)
+    if act_code is None:
+        _refuse(f"linear_int8: unknown activation {act!r}")
+    if out_dtype is None:
+        out_dtype = x.dtype
+    out_code = _DTYPE_CODES.get(out_dtype)
+    if out_code is None:
+        _refuse("linear_int8: out_dtype must be float32 or bfloat16")
+    if grad and _tracking():
+        _refuse("linear_int8 has no backward pass: call it under torch.no_grad()")
+    at = _device_of(x, weight, weight_scale, bias)
     bias = _float_vector(bias)
-    xd = _rows_of(x.detach())
-    w = weight if weight.stride(1) == 1 or k == 1 else weight.contiguous()
-    s = weight_scale.detach().contiguous()
-    m = xd.shape[0]
-    lib = nv.lib()
-    out = torch.empty(*x.shape[:-1], n, dtype=out_dtype, device=x.device)
-    ws_bytes = lib.spmi_linear_i8_workspace_bytes(m, k, n)
-    with torch.cuda.device(x.device):
-        ws = _workspace(ws_bytes, x.device)
-        nv.check(lib.spmi_linear_i8(nv.ptr(xd), code, xd.stride(0), m, k, nv.ptr(w), w.stride(0), nv.ptr(s), n,
-                                    nv.ptr(bias), _ACT_CODES[act], float(slope), nv.ptr(out),
-                                    _DTYPE_CODES[out_dtype], n, nv.ptr(ws), ws_bytes, nv.stream()), "spmi_linear_i8")
+    xr, w, s = _rows_of(x), _units_last(weight), _float_vector(weight_scale)
+    m = xr.shape[0]
+    out = _empty(*x.shape[:-1], n, dtype=out_dtype, device=x.device)
+    ws_bytes = nv.lib().spmi_linear_i8_workspace_bytes(m, k, n)
+    ws = _workspace(ws_bytes, x.device)
+    _launch("spmi_linear_i8", at, xr.data_ptr(), code, xr.stride(0), m, k, w.data_ptr(), w.stride(0), s.data_ptr(), n,
+            _ptr(bias), act_code, slope, out.data_ptr(), out_code, n, _ptr(ws), ws_bytes)
     return out
