@@ -728,7 +728,8 @@ int spmi_gated_step(const void* gates, int dtype, int64_t ldg, float* h_mem, int
  * with the quotient and the product of q rounded to float32 and the sum exact (K <= 131072).  A
  * row of x with a value that is not finite comes out as NaN (its q are 0, its scale NaN).
  * spmi_quantize_rows_i8 gives q and s alone: applied to a weight [N, K] it makes w and w_scale.
- * x and out are float32 or bfloat16; rows of x, w and out have strides in values and any alignment.
+ * x and out are float32 or bfloat16; rows of x, w and out have strides in values (of x and out below
+ * 2^24) and any alignment.
  * ---------------------------------------------------------------------- */
 int spmi_quantize_rows_i8(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, int8_t* q, int64_t ldq,
                           float* scale, void* stream);

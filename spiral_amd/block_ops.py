@@ -24,6 +24,8 @@ _DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1}
 LAYER_NORM_MAX_WIDTH = 16384  # spmi_layer_norm_max_width()
 INT8_MAX_INNER = 131072       # 127^2 times this still fits the 32-bit sums
 
+_INT8_MAX_STRIDE = 1 << 24     # values from one row to the next, in x and in the result
+
 _tracking = torch.is_grad_enabled
 _empty = torch.empty
 
@@ -376,6 +378,8 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     if weight.dim() != 2 or weight.dtype != torch.int8:
         _refuse(f"linear_int8: weight must be int8 [N, K], got {weight.dtype} {tuple(weight.shape)}")
     n, k = weight.shape
+    if n >= _INT8_MAX_STRIDE:
+        _refuse(f"linear_int8: {n} output channels are too many (below {_INT8_MAX_STRIDE})")
     if x.dim() < 1 or x.shape[-1] != k or not 1 <= k <= INT8_MAX_INNER:
         _refuse(f"linear_int8: x {tuple(x.shape)} does not fit a weight {tuple(weight.shape)}")
     if weight_scale.shape != (n,) or weight_scale.dtype != _F32:
@@ -399,6 +403,8 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     at = _device_of(x, weight, weight_scale, bias)
     bias = _float_vector(bias)
     xr, w, s = _rows_of(x), _units_last(weight), _float_vector(weight_scale)
+    if xr.stride(0) >= _INT8_MAX_STRIDE:
+        xr = xr.contiguous()
     m = xr.shape[0]
     out = _empty(*x.shape[:-1], n, dtype=out_dtype, device=x.device)
     ws_bytes = nv.lib().spmi_linear_i8_workspace_bytes(m, k, n)
