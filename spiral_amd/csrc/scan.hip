@@ -33,16 +33,18 @@ namespace {
 using namespace spmi;
 
 constexpr int kThreads = 256;
-constexpr int kFwdSteps = 8;   // steps a thread holds in registers
-constexpr int kBwdSteps = 4;
+// Steps a thread holds in registers, walking and as one of the strands.
+constexpr int kFwdSteps = 4;
+constexpr int kBwdWalkSteps = 4;
+constexpr int kBwdSteps = 2;
 constexpr int kLanes = 32;     // shape of a workgroup over few channels: lanes x strands
 constexpr int kStrands = kThreads / kLanes;
 // Threads (of four units) from which the steps are walked by one thread each: one wave per SIMD.
 constexpr int64_t kManyLanes = 65536;
 // Up to this many steps there is nothing to share among the strands.
 constexpr int64_t kFewSteps = 16;
-constexpr int64_t kTargetGroups = 512;  // workgroups wanted before the steps are split further
-constexpr int64_t kMaxSplits = 256;
+constexpr int64_t kTargetGroups = 2048;  // workgroups wanted before the steps are split further
+constexpr int64_t kMaxSplits = 512;
 
 struct ScanArgs {
   const void* gates;   // [T, N, 2H]: z, then c
@@ -97,8 +99,9 @@ struct Place {
 
 // Forward.  C lanes x S strands; MAPS: only the map of the split is wanted.
 template <typename T, int C, int S, bool MAPS>
-__global__ __launch_bounds__(kThreads) void scan_fwd_kernel(ScanArgs p) {
+__global__ __launch_bounds__(kThreads, S > 1 ? 4 : 1) void scan_fwd_kernel(ScanArgs p) {
   constexpr int L = kFwdSteps;
+  constexpr bool STREAM = S == 1;  // a split sequence is read twice, the second time from the caches
   static_assert(C * S == kThreads, "lanes x strands");
   __shared__ float4 meet[S > 1 ? 2 : 1][S][2][S > 1 ? C : 1];
   const int lane = threadIdx.x % C, strand = threadIdx.x / C;
@@ -111,21 +114,22 @@ __global__ __launch_bounds__(kThreads) void scan_fwd_kernel(ScanArgs p) {
   const T* gates = static_cast<const T*>(p.gates) + at.n * p.gates_n + at.c;
   const uint8_t* active = p.active ? p.active + at.n * p.active_n : nullptr;
 
+  // Loads without a condition around them, so that those of all steps are in flight together: steps past
+  // the end read the last one again, lanes past the end the first node's.  `on` says what counts.
   float a[L][4], b[L][4];
   bool on[L];
   auto fetch = [&](int64_t t0) {
+    unsigned act[L];
 #pragma unroll
     for (int i = 0; i < L; ++i) {
-      const int64_t t = t0 + strand * L + i;
-      on[i] = at.there && t < t_end;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) a[i][k] = b[i][k] = 0.0f;
-      if (on[i]) {
-        load4_upto(gates + t * p.gates_t, at.left, 0.0f, a[i]);
-        load4_upto(gates + t * p.gates_t + p.H, at.left, 0.0f, b[i]);
-        if (active) on[i] = active[t * p.active_t] != 0;
-      }
+      int64_t t = t0 + strand * L + i;
+      t = t < t_end ? t : t_end - 1;
+      act[i] = active ? active[t * p.active_t] : 1u;
+      load4_upto<STREAM>(gates + t * p.gates_t, at.left, 0.0f, a[i]);
+      load4_upto<STREAM>(gates + t * p.gates_t + p.H, at.left, 0.0f, b[i]);
     }
+#pragma unroll
+    for (int i = 0; i < L; ++i) on[i] = t0 + strand * L + i < t_end && act[i] != 0;
   };
   // z, c -> the step's map (a, (1 - a) c)
   auto to_maps = [&]() {
@@ -140,7 +144,7 @@ __global__ __launch_bounds__(kThreads) void scan_fwd_kernel(ScanArgs p) {
       }
   };
 
-  fetch(t_begin);
+  if (t_begin < t_end) fetch(t_begin);
 
   // the state the split starts from
   float h[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -155,7 +159,7 @@ __global__ __launch_bounds__(kThreads) void scan_fwd_kernel(ScanArgs p) {
         float4 P = make_float4(1, 1, 1, 1), Q = make_float4(0, 0, 0, 0);
         if (at.there) {
           const float* m = p.maps + channel * 4;
-#pragma unroll 4
+#pragma unroll 8
           for (int k = k0; k < k1; ++k) {
             const float4 pk = *reinterpret_cast<const float4*>(m + (2 * k) * lanes4);
             const float4 qk = *reinterpret_cast<const float4*>(m + (2 * k + 1) * lanes4);
@@ -194,7 +198,7 @@ __global__ __launch_bounds__(kThreads) void scan_fwd_kernel(ScanArgs p) {
       meet[turn][strand][0][lane] = make_float4(P[0], P[1], P[2], P[3]);
       meet[turn][strand][1][lane] = make_float4(Q[0], Q[1], Q[2], Q[3]);
       __syncthreads();
-#pragma unroll
+#pragma unroll 2
       for (int s = 0; s < S; ++s) {
         if (s == strand) {
 #pragma unroll
@@ -219,7 +223,7 @@ __global__ __launch_bounds__(kThreads) void scan_fwd_kernel(ScanArgs p) {
         const int64_t t = t0 + strand * L + i;
 #pragma unroll
         for (int k = 0; k < 4; ++k) start[k] = __builtin_fmaf(a[i][k], start[k], b[i][k]);
-        if (at.there && t < t_end) store4_upto(out + t * p.h_t, at.left, start);
+        if (at.there && t < t_end) store4_upto<true>(out + t * p.h_t, at.left, start);
       }
       if constexpr (S == 1) {
 #pragma unroll
@@ -243,8 +247,9 @@ __global__ __launch_bounds__(kThreads) void scan_fwd_kernel(ScanArgs p) {
 // Backward, from the last step down: strand 0 has the latest steps of a tile, split 0 the latest
 // steps of all.
 template <typename T, int C, int S, bool MAPS>
-__global__ __launch_bounds__(kThreads) void scan_bwd_kernel(ScanArgs p) {
-  constexpr int L = kBwdSteps;
+__global__ __launch_bounds__(kThreads, S > 1 ? 4 : 1) void scan_bwd_kernel(ScanArgs p) {
+  constexpr int L = S == 1 ? kBwdWalkSteps : kBwdSteps;
+  constexpr bool STREAM = S == 1;
   static_assert(C * S == kThreads, "lanes x strands");
   __shared__ float4 meet[S > 1 ? 2 : 1][S][2][S > 1 ? C : 1];
   const int lane = threadIdx.x % C, strand = threadIdx.x / C;
@@ -263,29 +268,45 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(ScanArgs p) {
   float z[L][4], c[L][4], gv[L][4], hp[L][4];
   bool on[L];
   auto fetch = [&](int64_t u0) {
+    unsigned act[L];
 #pragma unroll
     for (int i = 0; i < L; ++i) {
-      const int64_t u = u0 + strand * L + i, t = p.T - 1 - u;
-      on[i] = at.there && u < u_end;
+      int64_t u = u0 + strand * L + i;
+      u = u < u_end ? u : u_end - 1;
+      const int64_t t = p.T - 1 - u;
+      act[i] = active ? active[t * p.active_t] : 1u;
+      load4_upto<STREAM>(gates + t * p.gates_t, at.left, 0.0f, z[i]);
+      if (p.g) {
+        load4_upto<STREAM>(g + t * p.g_t, at.left, 0.0f, gv[i]);
+      } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) z[i][k] = c[i][k] = gv[i][k] = hp[i][k] = 0.0f;
-      if (on[i]) {
-        load4_upto(gates + t * p.gates_t, at.left, 0.0f, z[i]);
-        if (p.g) load4_upto(g + t * p.g_t, at.left, 0.0f, gv[i]);
-        if constexpr (!MAPS) {
-          load4_upto(gates + t * p.gates_t + p.H, at.left, 0.0f, c[i]);
-          if (t > 0) {
-            load4_upto(h + (t - 1) * p.h_t, at.left, 0.0f, hp[i]);
-          } else if (p.h0) {
-            load4_upto(p.h0 + at.n * p.h0_n + at.c, at.left, 0.0f, hp[i]);
-          }
+        for (int k = 0; k < 4; ++k) gv[i][k] = 0.0f;
+      }
+      if constexpr (!MAPS) {
+        load4_upto<STREAM>(gates + t * p.gates_t + p.H, at.left, 0.0f, c[i]);
+        // the state before the step; before the first one it is h0, put in below
+        if (p.T > 1) load4_upto<STREAM>(h + (t > 0 ? t - 1 : 0) * p.h_t, at.left, 0.0f, hp[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      const int64_t u = u0 + strand * L + i;
+      on[i] = u < u_end && act[i] != 0;
+      if constexpr (!MAPS) {
+        if (u == p.T - 1) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) hp[i][k] = 0.0f;
+          if (p.h0) load4_upto(p.h0 + at.n * p.h0_n + at.c, at.left, 0.0f, hp[i]);
         }
-        if (active) on[i] = active[t * p.active_t] != 0;
+      }
+      if (u >= u_end) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) gv[i][k] = 0.0f;  // a step that is not there passes e on as it is
       }
     }
   };
 
-  fetch(u_begin);
+  if (u_begin < u_end) fetch(u_begin);
 
   float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   float prod[4] = {1.0f, 1.0f, 1.0f, 1.0f};  // MAPS
@@ -298,7 +319,7 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(ScanArgs p) {
         float4 P = make_float4(1, 1, 1, 1), Q = make_float4(0, 0, 0, 0);
         if (at.there) {
           const float* m = p.maps + channel * 4;
-#pragma unroll 4
+#pragma unroll 8
           for (int k = k0; k < k1; ++k) {
             const float4 pk = *reinterpret_cast<const float4*>(m + (2 * k) * lanes4);
             const float4 qk = *reinterpret_cast<const float4*>(m + (2 * k + 1) * lanes4);
@@ -343,7 +364,7 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(ScanArgs p) {
       meet[turn][strand][0][lane] = make_float4(P[0], P[1], P[2], P[3]);
       meet[turn][strand][1][lane] = make_float4(Q[0], Q[1], Q[2], Q[3]);
       __syncthreads();
-#pragma unroll
+#pragma unroll 2
       for (int s = 0; s < S; ++s) {
         if (s == strand) {
 #pragma unroll
@@ -375,8 +396,8 @@ __global__ __launch_bounds__(kThreads) void scan_bwd_kernel(ScanArgs p) {
           start[k] = a[i][k] * d;
         }
         if (p.dgates && at.there && u < u_end) {
-          store4_upto(out + t * p.dg_t, at.left, dz);
-          store4_upto(out + t * p.dg_t + p.H, at.left, dc);
+          store4_upto<true>(out + t * p.dg_t, at.left, dz);
+          store4_upto<true>(out + t * p.dg_t + p.H, at.left, dc);
         }
       }
       if constexpr (S == 1) {
