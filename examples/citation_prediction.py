@@ -1,7 +1,10 @@
 """Citation-count prediction on a discrete-time dynamic graph, the pipeline of the reference's
 examples/torch/citation_prediction.py with `spiro` replaced by `spiral_amd`: a GCN / SGCN / GAT /
 GraphSage encoder per snapshot, a GRU / LSTM / RNN over per-node memory, an MLP head; labels are
-the citation counts of the next snapshot; Adam, MSE, one backward pass per snapshot.
+the citation counts of the next snapshot; Adam, MSE, one backward pass per snapshot.  `--rnn glru`
+takes the gated linear recurrence as the cell, and with `--window W` trains it through W snapshots
+at a time (one scan and one backward pass for all of them); `--int8` then serves the test
+snapshot with 8-bit projections.
 
     python examples/citation_prediction.py                     # synthetic citation graph
     python examples/citation_prediction.py --dataset ogbn-arxiv  # needs the `ogb` package and its data
@@ -24,7 +27,7 @@ from spiral_amd.core.config import set_backend  # noqa: E402
 set_backend(PYTORCH)
 from spiral_amd.automl.model_assembler import assembler  # noqa: E402
 from spiral_amd.dtdg.dataloader import ogb_dataset, preprocess_citation_graph, supported_ogb_datasets  # noqa: E402
-from spiral_amd.dtdg.models.decoder.sequentialDecoders import GRU, LSTM, RNN  # noqa: E402
+from spiral_amd.dtdg.models.decoder.sequentialDecoders import GLRU, GRU, LSTM, RNN  # noqa: E402
 from spiral_amd.dtdg.models.decoder.simpleDecoders import MLP  # noqa: E402
 from spiral_amd.dtdg.models.encoder.implicitTimeEncoder.staticGraphEncoder import GAT, GCN, SGCN, GraphSage  # noqa: E402
 
@@ -55,15 +58,34 @@ def build_model(args, in_dim: int, n_nodes: int):
     else:
         gnn = GraphSage("gcn", in_dim, args.hidden, depth=args.gnn_layers, activation=act)
     head = MLP(args.rnn_hidden, [10, 20, 10, 5])
-    cell = {"gru": GRU, "lstm": LSTM, "rnn": RNN}[args.rnn]
+    cell = {"gru": GRU, "lstm": LSTM, "rnn": RNN, "glru": GLRU}[args.rnn]
     return assembler(gnn, cell(args.hidden, args.rnn_hidden, n_nodes, args.rnn_layers, head))
+
+
+def window_step(model, graph, first: int, steps: int):
+    """Prediction and label of every node of the snapshots first .. first + steps - 1, the recurrence
+    tracked through all of them.  The nodes of a snapshot are the first rows of the later ones, so
+    the embeddings are stacked with the rows of nodes that are not there yet marked as inactive."""
+    embs, labels = [], []
+    for t in range(first, first + steps):
+        snapshot, ids = graph.dispatcher(t)
+        nxt, _ = graph.dispatcher(t + 1)
+        embs.append(model.encoder((snapshot, ids))[0])
+        labels.append(nxt.node_feature()[: snapshot.num_nodes(), -1].float())
+    n = embs[-1].shape[0]
+    stacked = torch.stack([F.pad(e, (0, 0, 0, n - e.shape[0])) for e in embs])
+    counts = torch.tensor([e.shape[0] for e in embs], device=stacked.device)
+    active = torch.arange(n, device=stacked.device)[None, :] < counts[:, None]
+    return model.decoder.forward_sequence(stacked, active=active).squeeze(), torch.cat(labels)
 
 
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--dataset", default="synthetic", choices=["synthetic"] + supported_ogb_datasets())
     ap.add_argument("--gnn", default="gcn", choices=["gcn", "sgcn", "gat", "sage"])
-    ap.add_argument("--rnn", default="gru", choices=["gru", "lstm", "rnn"])
+    ap.add_argument("--rnn", default="gru", choices=["gru", "lstm", "rnn", "glru"])
+    ap.add_argument("--window", type=int, default=1, help="snapshots trained through at a time (glru)")
+    ap.add_argument("--int8", action="store_true", help="8-bit projections for the last test (glru)")
     ap.add_argument("--gnn-layers", type=int, default=2)
     ap.add_argument("--rnn-layers", type=int, default=2)
     ap.add_argument("--hidden", type=int, default=32)
@@ -74,6 +96,8 @@ def main():
     ap.add_argument("--edges", type=int, default=200_000)
     ap.add_argument("--years", type=int, default=12)
     args = ap.parse_args()
+    if (args.window > 1 or args.int8) and args.rnn != "glru":
+        ap.error("--window and --int8 need --rnn glru")
     dev = torch.device("cuda:0")
 
     if args.dataset == "synthetic":
@@ -93,16 +117,21 @@ def main():
         model.decoder.reset_memory_state()
         model.train()
         t0 = time.perf_counter()
-        for t in range(first, n_snapshot - 2):
-            snapshot, ids = graph.dispatcher(t)
-            nxt, _ = graph.dispatcher(t + 1)
+        for t in range(first, n_snapshot - 2, args.window):
             opt.zero_grad()
-            predict = model((snapshot, ids))
-            label = nxt.node_feature()[: snapshot.num_nodes(), -1].float()
+            if args.window > 1:
+                predict, label = window_step(model, graph, t, min(args.window, n_snapshot - 2 - t))
+            else:
+                snapshot, ids = graph.dispatcher(t)
+                nxt, _ = graph.dispatcher(t + 1)
+                predict = model((snapshot, ids))
+                label = nxt.node_feature()[: snapshot.num_nodes(), -1].float()
             loss = F.mse_loss(predict.squeeze(), label)
             loss.backward()
             opt.step()
         model.eval()
+        if args.int8 and epoch == args.epochs - 1:
+            model.decoder.to_int8()
         with torch.no_grad():
             snapshot, ids = graph.dispatcher(n_snapshot - 2)
             nxt, _ = graph.dispatcher(n_snapshot - 1)

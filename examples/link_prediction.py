@@ -29,7 +29,7 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 from spiral_amd.automl.evaluate import link_prediction_mrr  # noqa: E402
 from spiral_amd.automl.model_assembler import assembler  # noqa: E402
 from spiral_amd.automl.prepare_dataset import LABEL, TARGET, prepare_edge_task  # noqa: E402
-from spiral_amd.dtdg.models.decoder.sequentialDecoders import GRU, LSTM, RNN  # noqa: E402
+from spiral_amd.dtdg.models.decoder.sequentialDecoders import GLRU, GRU, LSTM, RNN  # noqa: E402
 from spiral_amd.dtdg.models.decoder.simpleDecoders import MLP  # noqa: E402
 from spiral_amd.dtdg.models.encoder.implicitTimeEncoder.staticGraphEncoder import GAT, GCN, SGCN, GraphSage  # noqa: E402
 from spiral_amd.dtdg.types import VEInvariantDTDG  # noqa: E402
@@ -69,7 +69,7 @@ def masked_snapshot(graph, t):
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--gnn", default="gcn", choices=["gcn", "sgcn", "gat", "sage"])
-    ap.add_argument("--rnn", default="gru", choices=["gru", "lstm", "rnn"])
+    ap.add_argument("--rnn", default="gru", choices=["gru", "lstm", "rnn", "glru"])
     ap.add_argument("--hidden", type=int, default=32)
     ap.add_argument("--output-dim", type=int, default=10)
     ap.add_argument("--epochs", type=int, default=5)
@@ -101,7 +101,7 @@ def main():
     else:
         gnn = GraphSage("gcn", in_dim, args.hidden, activation=act)
     head = MLP(2 * args.output_dim, [args.hidden, 20, 10, 5], activation="sigmoid")
-    cell = {"gru": GRU, "lstm": LSTM, "rnn": RNN}[args.rnn]
+    cell = {"gru": GRU, "lstm": LSTM, "rnn": RNN, "glru": GLRU}[args.rnn]
     model = assembler(gnn, cell(args.hidden, args.output_dim, eval_snapshot.num_nodes(), 2, head)).to(dev)
     opt = torch.optim.Adam(model.parameters(), lr=1e-3, eps=1e-8)
     loss_fn = swapped_bce if args.reference_loss_order else F.binary_cross_entropy
