@@ -193,9 +193,12 @@ struct RowsArgs {
 // the block fit 32 bits).
 template <typename OUT>
 struct Block {
-  static constexpr int kStream = 2;  // nontemporal: outputs are not read again by the kernel
   __amdgpu_buffer_rsrc_t rsrc;
   int ld;  // bytes
+  // The rows' 32 neighbouring outputs are whole 64-byte pieces of memory.  Only then are they stored as a
+  // stream: pieces written in parts have to meet in the cache (58998 x 64 -> 431 in float32 takes 87 us
+  // with the mark, 31 without).
+  bool lines;
   // The address goes through the first lane: the compiler then knows it for a scalar and does not
   // loop over the lanes for each store.
   static __device__ OUT* scalar(OUT* p) {
@@ -206,12 +209,15 @@ struct Block {
   }
   __device__ Block(OUT* base, int64_t ldo)
       : rsrc(__builtin_amdgcn_make_buffer_rsrc(scalar(base), 0, static_cast<int>(32 * ldo * sizeof(OUT)), 0x00027000)),
-        ld(static_cast<int>(ldo * sizeof(OUT))) {}
+        ld(static_cast<int>(ldo * sizeof(OUT))),
+        lines(((reinterpret_cast<uint64_t>(base) | static_cast<uint64_t>(ldo * sizeof(OUT))) & 63) == 0) {}
+  // STREAM: marked as not read again soon (2 = nontemporal).
+  template <bool STREAM>
   __device__ __forceinline__ void store(OUT v, unsigned lane_off, int row) const {
     if constexpr (sizeof(OUT) == 4)
-      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), rsrc, lane_off, row * ld, kStream);
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), rsrc, lane_off, row * ld, STREAM ? 2 : 0);
     else
-      __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), rsrc, lane_off, row * ld, kStream);
+      __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), rsrc, lane_off, row * ld, STREAM ? 2 : 0);
   }
 };
 
@@ -252,14 +258,13 @@ __device__ __forceinline__ void finish16(const i32x16& acc, const float (&sm)[16
 #pragma unroll
     for (int r = 0; r < 16; ++r) y[r] = y[r] < 0.0f ? y[r] * slope : y[r];
   }
-  const auto put = [&](int r) { to.store(static_cast<OUT>(y[r]), lane_off, 8 * (r / 4) + r % 4); };
-  if (left >= 32) {
+  if (left >= 32 && to.lines) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) put(r);
+    for (int r = 0; r < 16; ++r) to.template store<true>(static_cast<OUT>(y[r]), lane_off, 8 * (r / 4) + r % 4);
   } else {
 #pragma unroll
     for (int r = 0; r < 16; ++r)
-      if (8 * (r / 4) + r % 4 < left) put(r);
+      if (8 * (r / 4) + r % 4 < left) to.template store<false>(static_cast<OUT>(y[r]), lane_off, 8 * (r / 4) + r % 4);
   }
 }
 
@@ -468,21 +473,33 @@ __global__ __launch_bounds__(RowsShape<KP>::NW * 64, 2) void rows_i8_kernel(Rows
   const int64_t row0 = (static_cast<int64_t>(blockIdx.x) * S::NW + wave) * 32;
   const bool full = row0 + 32 <= p.M;
   const T* const x0 = static_cast<const T*>(p.x) + row0 * p.ldx;
-  const unsigned x_off = static_cast<unsigned>(sub * static_cast<int>(p.ldx) + c) * sizeof(T);
+  const int last_row = full ? 31 : static_cast<int>(p.M - 1 - row0);  // may be negative: rows before the wave's
   float v[LOADS][R][4];
   auto fetch = [&](int r0) {  // rows r0 .. r0 + BROWS of the wave's 32
-    if (full && p.K % 4 == 0) {
-      // lanes past the end of a row read its start and forget it
+    // Loads without a condition around them, so that all are in flight together: rows past the end read
+    // the last row again, and a lane whose four values pass the end of the row reads the row's last four
+    // and moves them down.
+    if (p.K >= 4) {
 #pragma unroll
-      for (int b = 0; b < LOADS; ++b)
+      for (int b = 0; b < LOADS; ++b) {
+        int row = r0 + b * RPL + sub;
+        row = row <= last_row ? row : last_row;
+        const T* const src = x0 + row * p.ldx;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const bool in = r * 256 + c < p.K;
-          const char* const src = reinterpret_cast<const char*>(x0 + (r0 + b * RPL) * p.ldx);
-          load4<true>(reinterpret_cast<const T*>(src + (in ? x_off + r * 256 * sizeof(T) : x_off - c * sizeof(T))), v[b][r]);
+          const int k = r * 256 + c, from = k <= p.K - 4 ? k : p.K - 4, by = k - from;
+          load4<true>(src + from, v[b][r]);
+          float (&t)[4] = v[b][r];
+          if (p.K % 4) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[b][r][i] = in ? v[b][r][i] : 0.0f;
+            for (int i = 0; i < 4; ++i) t[i] = (by & 2) ? (i < 2 ? t[i + 2] : 0.0f) : t[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t[i] = (by & 1) ? (i < 3 ? t[i + 1] : 0.0f) : t[i];
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) t[i] = by < 4 ? t[i] : 0.0f;
         }
+      }
     } else {
 #pragma unroll
       for (int b = 0; b < LOADS; ++b)
@@ -491,8 +508,8 @@ __global__ __launch_bounds__(RowsShape<KP>::NW * 64, 2) void rows_i8_kernel(Rows
 #pragma unroll
           for (int i = 0; i < 4; ++i) v[b][r][i] = 0.0f;
           const int k = r * 256 + c;
-          if (row0 + r0 + b * RPL + sub < p.M && k < p.K)
-            load4_upto<true>(x0 + (r0 + b * RPL + sub) * p.ldx + k, p.K - k, 0.0f, v[b][r]);
+          if (r0 + b * RPL + sub <= last_row && k < p.K)
+            load4_upto(x0 + (r0 + b * RPL + sub) * p.ldx + k, p.K - k, 0.0f, v[b][r]);
         }
     }
   };
@@ -806,7 +823,7 @@ int launch_few(const FewArgs& a, hipStream_t st) {
 }
 // Whole numbers that every workgroup of few_i8_kernel makes for itself.
 constexpr int64_t kFewMade = 16384;
-bool few_made(int64_t M, int64_t K) { return M <= kFewRows && M * K <= kFewMade; }
+bool few_made(int64_t M, int64_t K) { return M <= 16 && M * K <= kFewMade; }
 
 int check_rows(const char* what, int dtype, int64_t M, int64_t K) {
   SPMI_REQUIRE(dtype == SPMI_DTYPE_F32 || dtype == SPMI_DTYPE_BF16, SPMI_ERR_INVALID_ARG, "%s: dtype %d", what, dtype);
