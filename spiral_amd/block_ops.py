@@ -109,12 +109,11 @@ class _Operator(torch.autograd.Function):
 
 
 # --------------------------------------------------------------------------- layer norm
-def _layer_norm_fwd(x, weight, bias, eps, code, at, keep):
-    xr = _rows_of(x)
+def _layer_norm_fwd(xr, shape, weight, bias, eps, code, at, keep):
     m, d = xr.shape
     w, b = _float_vector(weight), _float_vector(bias)
-    y = _empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = _empty(m, 2, dtype=_F32, device=x.device) if keep else None
+    y = _empty(shape, dtype=xr.dtype, device=xr.device)
+    stats = _empty(m, 2, dtype=_F32, device=xr.device) if keep else None
     _launch("spmi_layer_norm_fwd", at, xr.data_ptr(), code, xr.stride(0), m, d, _ptr(w), _ptr(b), eps, y.data_ptr(),
             d, _ptr(stats))
     return y, stats
@@ -123,27 +122,38 @@ def _layer_norm_fwd(x, weight, bias, eps, code, at, keep):
 class _LayerNorm(_Operator):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, code, at):
-        y, stats = _layer_norm_fwd(x, weight, bias, eps, code, at, True)
+        xr = _rows_of(x)
+        y, stats = _layer_norm_fwd(xr, x.shape, weight, bias, eps, code, at, True)
         ctx.save_for_backward(x, weight, stats)
-        ctx.plain = (code, at, None if bias is None else bias.dtype)
+        m, d = xr.shape
+        # what the backward pass would otherwise ask for again, in a thread that is slow at asking
+        ctx.plain = (code, at, m, d, xr.stride(0) if xr.data_ptr() == x.data_ptr() else None,
+                     nv.lib().spmi_layer_norm_bwd_workspace_bytes(m, d), None if bias is None else bias.dtype)
         return y
 
     @staticmethod
     def gradients(ctx, g):
         x, weight, stats = ctx.saved_tensors
-        code, at, bias_dtype = ctx.plain
+        code, at, m, d, ld, ws_bytes, bias_dtype = ctx.plain
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        xr, gr = _rows_of(x), _rows_of(g)
-        m, d = xr.shape
         dev = x.device
+        if ld is None:
+            x = _rows_of(x)
+            ld = x.stride(0)
+        ldg = d
+        shape = g.shape
+        if not g.is_contiguous():
+            g = _rows_of(g)
+            ldg = g.stride(0)
         w = _float_vector(weight)
-        dx = _empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+        dx = _empty(shape, dtype=x.dtype, device=dev) if need_x else None
         dw = _empty(d, dtype=_F32, device=dev) if need_w else None
         db = _empty(d, dtype=_F32, device=dev) if need_b else None
-        ws_bytes = nv.lib().spmi_layer_norm_bwd_workspace_bytes(m, d) if need_w or need_b else 0
+        if not (need_w or need_b):
+            ws_bytes = 0
         ws = _workspace(ws_bytes, dev)
-        _launch("spmi_layer_norm_bwd", at, xr.data_ptr(), gr.data_ptr(), code, xr.stride(0), gr.stride(0), m, d,
-                _ptr(w), stats.data_ptr(), _ptr(dx), d, _ptr(dw), _ptr(db), _ptr(ws), ws_bytes)
+        _launch("spmi_layer_norm_bwd", at, x.data_ptr(), g.data_ptr(), code, ld, ldg, m, d, _ptr(w), stats.data_ptr(),
+                _ptr(dx), d, _ptr(dw), _ptr(db), _ptr(ws), ws_bytes)
         if need_w and weight.dtype != _F32:
             dw = dw.to(weight.dtype)
         if need_b and bias_dtype != _F32:
@@ -176,7 +186,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     at = _device_of(x, weight, bias)
     if grad and _tracking():
         return _LayerNorm.apply(x, weight, bias, eps, code, at)
-    return _layer_norm_fwd(x, weight, bias, eps, code, at, False)[0]
+    return _layer_norm_fwd(_rows_of(x), x.shape, weight, bias, eps, code, at, False)[0]
 
 
 # --------------------------------------------------------------------------- gated linear recurrence
@@ -187,59 +197,61 @@ def _step_strides(t: Optional[torch.Tensor], batch_first: bool) -> Tuple[int, in
     return (t.stride(1), t.stride(0)) if batch_first else (t.stride(0), t.stride(1))
 
 
-def _scan_head(gates, h0, active, batch_first, code, h):
-    """The arguments both directions begin with."""
+def _scan_sizes(gates, h0, active, batch_first, h):
+    """The numbers both directions take: strides of gates, h0, active and h, and T, N, H."""
     n, t = gates.shape[:2] if batch_first else (gates.shape[1], gates.shape[0])
-    return (gates.data_ptr(), code, *_step_strides(gates, batch_first), _ptr(h0), 0 if h0 is None else h0.stride(0),
-            _ptr(active), *_step_strides(active, batch_first), t, n, gates.shape[2] // 2, h.data_ptr(),
-            *_step_strides(h, batch_first))
+    return (_step_strides(gates, batch_first), 0 if h0 is None else h0.stride(0), _step_strides(active, batch_first),
+            (t, n, gates.shape[2] // 2), _step_strides(h, batch_first))
 
 
-def _scan_bwd(gates, h0, active, batch_first, code, at, h, g, g_last, dgates, dh0):
-    head = _scan_head(gates, h0, active, batch_first, code, h)
-    ws_bytes = nv.lib().spmi_gated_scan_bwd_workspace_bytes(*head[9:12])
+def _scan_bwd(gates, h0, active, batch_first, code, at, h, g, g_last, dgates, dh0, sizes, ws_bytes):
+    of_gates, of_h0, of_active, tnh, of_h = sizes
     ws = _workspace(ws_bytes, gates.device)
-    _launch("spmi_gated_scan_bwd", at, *head, _ptr(g), *_step_strides(g, batch_first), _ptr(g_last),
+    _launch("spmi_gated_scan_bwd", at, gates.data_ptr(), code, *of_gates, _ptr(h0), of_h0, _ptr(active), *of_active,
+            *tnh, h.data_ptr(), *of_h, _ptr(g), *_step_strides(g, batch_first), _ptr(g_last),
             0 if g_last is None else g_last.stride(0), _ptr(dgates), *_step_strides(dgates, batch_first), _ptr(dh0),
             _ptr(ws), ws_bytes)
 
 
 def _scan_fwd(gates, h0, active, batch_first, code, at):
     gates = _units_last(gates)
-    n, t = gates.shape[:2] if batch_first else (gates.shape[1], gates.shape[0])
-    hd = gates.shape[2] // 2
     if h0 is not None:
         h0 = _units_last(h0)
-    h = _empty(*gates.shape[:2], hd, dtype=gates.dtype, device=gates.device)
-    last = _empty(n, hd, dtype=_F32, device=gates.device)
-    ws_bytes = nv.lib().spmi_gated_scan_fwd_workspace_bytes(t, n, hd)
-    ws = _workspace(ws_bytes, gates.device)
-    _launch("spmi_gated_scan_fwd", at, *_scan_head(gates, h0, active, batch_first, code, h), last.data_ptr(),
-            _ptr(ws), ws_bytes)
-    return h, last
+    dev = gates.device
+    h = _empty(*gates.shape[:2], gates.shape[2] // 2, dtype=gates.dtype, device=dev)
+    sizes = _scan_sizes(gates, h0, active, batch_first, h)
+    of_gates, of_h0, of_active, tnh, of_h = sizes
+    last = _empty(tnh[1:], dtype=_F32, device=dev)
+    ws_bytes = nv.lib().spmi_gated_scan_fwd_workspace_bytes(*tnh)
+    ws = _workspace(ws_bytes, dev)
+    _launch("spmi_gated_scan_fwd", at, gates.data_ptr(), code, *of_gates, _ptr(h0), of_h0, _ptr(active), *of_active,
+            *tnh, h.data_ptr(), *of_h, last.data_ptr(), _ptr(ws), ws_bytes)
+    return h, last, sizes
 
 
 class _GatedScan(_Operator):
     @staticmethod
     def forward(ctx, gates, h0, active, batch_first, code, at):
-        h, last = _scan_fwd(gates, h0, active, batch_first, code, at)
+        h, last, sizes = _scan_fwd(gates, h0, active, batch_first, code, at)
         ctx.save_for_backward(gates, h0, active, h)
-        ctx.plain = (batch_first, code, at)
+        ctx.plain = (batch_first, code, at, sizes, nv.lib().spmi_gated_scan_bwd_workspace_bytes(*sizes[3]))
         ctx.set_materialize_grads(False)
         return h, last
 
     @staticmethod
     def gradients(ctx, g, g_last):
         gates, h0, active, h = ctx.saved_tensors
-        batch_first, code, at = ctx.plain
+        batch_first, code, at, sizes, ws_bytes = ctx.plain
         need_gates, need_h0 = ctx.needs_input_grad[:2]
         if g is None and g_last is None:
             return None, None, None, None, None, None
-        gates = _units_last(gates)
+        gates = _units_last(gates)  # the same copy as in forward, if it was one: sizes fit
+        if h0 is not None:
+            h0 = _units_last(h0)
         dgates = _empty(gates.shape, dtype=gates.dtype, device=gates.device) if need_gates else None
         dh0 = _empty(h0.shape, dtype=_F32, device=gates.device) if need_h0 else None
-        _scan_bwd(gates, None if h0 is None else _units_last(h0), active, batch_first, code, at, h,
-                  None if g is None else _units_last(g), None if g_last is None else _units_last(g_last), dgates, dh0)
+        _scan_bwd(gates, h0, active, batch_first, code, at, h, None if g is None else _units_last(g),
+                  None if g_last is None else _units_last(g_last), dgates, dh0, sizes, ws_bytes)
         return dgates, dh0, None, None, None, None
 
 
@@ -273,7 +285,7 @@ def gated_scan(gates: torch.Tensor, h0: Optional[torch.Tensor] = None, active: O
     at = _device_of(gates, h0, active)
     if grad and _tracking():
         return _GatedScan.apply(gates, h0, active, batch_first, code, at)
-    return _scan_fwd(gates, h0, active, batch_first, code, at)
+    return _scan_fwd(gates, h0, active, batch_first, code, at)[:2]
 
 
 def _step_fwd(gates, h_mem, ids, mem_write, code, at, keep):
@@ -305,7 +317,9 @@ class _GatedStep(_Operator):
         gates, before = ctx.saved_tensors
         gates = _units_last(gates)
         dgates = _empty(gates.shape, dtype=gates.dtype, device=gates.device)
-        _scan_bwd(gates[None], before, None, False, *ctx.plain, before[None], None, _units_last(g), dgates[None], None)
+        m, h2 = gates.shape
+        sizes = ((0, gates.stride(0)), h2 // 2, (0, 0), (1, m, h2 // 2), (0, 0))
+        _scan_bwd(gates, before, None, False, *ctx.plain, before, None, _units_last(g), dgates[None], None, sizes, 0)
         return dgates, None, None, None, None, None
 
 

@@ -22,6 +22,7 @@ constexpr int kThreads = 256;
 #define WAIT_LOADS(n) (((n) & 15) | ((n) >> 4 << 14) | (7 << 4) | (15 << 8))
 // The same for LDS: all reads have returned.
 #define WAIT_LDS (15 | (3 << 14) | (7 << 4))
+constexpr int64_t kMaxGroups = 1 << 22;  // of kThreads: a grid holds less than 2^32 threads
 constexpr int64_t kMaxInner = 131072;
 constexpr int64_t kMaxStride = 1 << 24;  // of a row of x and of the output, in values
 // Smallest row maximum that is divided by: 127 / 2^-120 is still finite.
@@ -73,53 +74,54 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const T* __restrict_
                                                             int8_t* __restrict__ q, int64_t ldq, int width,
                                                             float* __restrict__ scale) {
   const int lane = threadIdx.x & 63;
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 6;
-  if (row >= M) return;
-  const T* const src = x + row * ldx;
-  int8_t* const dst = q + row * ldq;
-  unsigned top = 0;
-  float v[R > 0 ? R : 1][4];
-  if constexpr (R > 0) {
+  for (int64_t row = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 6; row < M;
+       row += (static_cast<int64_t>(gridDim.x) * kThreads) >> 6) {
+    const T* const src = x + row * ldx;
+    int8_t* const dst = q + row * ldq;
+    unsigned top = 0;
+    float v[R > 0 ? R : 1][4];
+    if constexpr (R > 0) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int c = r * 256 + lane * 4;
+      for (int r = 0; r < R; ++r) {
+        const int c = r * 256 + lane * 4;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[r][i] = 0.0f;
-      if (c < K) load4_upto<true>(src + c, K - c, 0.0f, v[r]);
-    }
+        for (int i = 0; i < 4; ++i) v[r][i] = 0.0f;
+        if (c < K) load4_upto<true>(src + c, K - c, 0.0f, v[r]);
+      }
 #pragma unroll
-    for (int r = 0; r < R; ++r) top = top_of(top, v[r]);
-  } else {
-#pragma unroll 4
-    for (int c = lane * 4; c < K; c += 256) {
-      load4_upto(src + c, K - c, 0.0f, v[0]);
-      top = top_of(top, v[0]);
-    }
-  }
-  top = group_top<64>(top);
-  float inv, s;
-  row_scale(top, inv, s);
-  if (lane == 0) scale[row] = s;
-  const auto put = [&](int c, const float (&t)[4]) {
-    const unsigned w = pack4(t, inv);
-    if (c + 4 <= width) {
-      __builtin_memcpy(dst + c, &w, 4);
+      for (int r = 0; r < R; ++r) top = top_of(top, v[r]);
     } else {
-#pragma unroll
-      for (int i = 0; i < 3; ++i)
-        if (c + i < width) dst[c + i] = static_cast<int8_t>(w >> (8 * i));
-    }
-  };
-  if constexpr (R > 0) {
-#pragma unroll
-    for (int r = 0; r < R; ++r) put(r * 256 + lane * 4, v[r]);
-  } else {
 #pragma unroll 4
-    for (int c = lane * 4; c < width; c += 256) {
+      for (int c = lane * 4; c < K; c += 256) {
+        load4_upto(src + c, K - c, 0.0f, v[0]);
+        top = top_of(top, v[0]);
+      }
+    }
+    top = group_top<64>(top);
+    float inv, s;
+    row_scale(top, inv, s);
+    if (lane == 0) scale[row] = s;
+    const auto put = [&](int c, const float (&t)[4]) {
+      const unsigned w = pack4(t, inv);
+      if (c + 4 <= width) {
+        __builtin_memcpy(dst + c, &w, 4);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[0][i] = 0.0f;
-      if (c < K) load4_upto(src + c, K - c, 0.0f, v[0]);
-      put(c, v[0]);
+        for (int i = 0; i < 3; ++i)
+          if (c + i < width) dst[c + i] = static_cast<int8_t>(w >> (8 * i));
+      }
+    };
+    if constexpr (R > 0) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) put(r * 256 + lane * 4, v[r]);
+    } else {
+#pragma unroll 4
+      for (int c = lane * 4; c < width; c += 256) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[0][i] = 0.0f;
+        if (c < K) load4_upto(src + c, K - c, 0.0f, v[0]);
+        put(c, v[0]);
+      }
     }
   }
 }
@@ -382,6 +384,7 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_i8_kernel(GemmArgs p) {
   };
   static_assert(ST >= 3, "the loads of a stage are waited for one stage early");
   asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(WAIT_LDS);  // the scales are there for everyone after the barrier
   if (ST - 1 <= stages) wait(std::integral_constant<int, ST - 2>{});
   else wait(std::integral_constant<int, 0>{});
   __builtin_amdgcn_s_barrier();
@@ -838,7 +841,7 @@ template <typename T>
 void launch_quantize(const void* x, int64_t ldx, int64_t M, int64_t K, int8_t* q, int64_t ldq, int64_t width,
                      float* scale, hipStream_t st) {
   const auto go = [&](auto r) {
-    quantize_kernel<T, decltype(r)::value><<<static_cast<unsigned>((M + 3) / 4), kThreads, 0, st>>>(
+    quantize_kernel<T, decltype(r)::value><<<static_cast<unsigned>((M + 3) / 4 < kMaxGroups ? (M + 3) / 4 : kMaxGroups), kThreads, 0, st>>>(
         static_cast<const T*>(x), ldx, M, static_cast<int>(K), q, ldq, static_cast<int>(width), scale);
   };
   if (width <= 256) go(std::integral_constant<int, 1>{});

@@ -25,6 +25,8 @@ constexpr int kThreads = 256;
 constexpr int64_t kMaxWidth = 16384;
 constexpr int kGather = 64;    // partial rows that are added up in a step of their own
 constexpr int kMaxLast = 512;  // partial rows that the last step takes
+constexpr int64_t kMaxParts = 1 << 20;   // partial rows in all
+constexpr int64_t kMaxGroups = 1 << 20;  // workgroups of a launch: a grid holds less than 2^32 threads
 
 struct FwdArgs {
   const void* x;
@@ -98,9 +100,9 @@ __device__ __forceinline__ void store_row(T* dst, int lane, int D, const float (
   }
 }
 
-// A group works on RU rows at a time.  The grid covers the rows once: workgroups that are handed out in
-// order keep the accesses in flight close together, where a resident grid that strides over the rows
-// lets its workgroups drift apart.
+// A group works on RU rows at a time.  The grid covers the rows once (the loop is for more rows than a
+// grid can hold): workgroups that are handed out in order keep the accesses in flight close together,
+// where a resident grid that strides over the rows lets its workgroups drift apart.
 template <typename T, int G, int R, int LO, int RU>
 __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_fwd_kernel(FwdArgs p) {
   constexpr bool WG = G > 64;
@@ -129,39 +131,42 @@ __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_fwd_kernel(Fwd
 #pragma unroll
       for (int i = 0; i < 4; ++i) b[r][i] = 0.0f;
   }
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (GROUPS * RU) + grp;
-  float v[RU][R][4];
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * (GROUPS * RU); first < p.M;
+       first += static_cast<int64_t>(gridDim.x) * (GROUPS * RU)) {
+    const int64_t row0 = first + grp;
+    float v[RU][R][4];
 #pragma unroll
-  for (int u = 0; u < RU; ++u) {
-    const int64_t row = row0 + u * GROUPS;  // past the end: the last row again, not stored
-    load_row<G, R, LO, true>(x + (row < p.M ? row : p.M - 1) * p.ldx, lane, p.D, 0.0f, v[u]);
-  }
-#pragma unroll
-  for (int u = 0; u < RU; ++u) {
-    const int64_t row = row0 + u * GROUPS;
-    float s = 0.0f;
-#pragma unroll
-    for (int r = 0; r < R; ++r) s += (v[u][r][0] + v[u][r][1]) + (v[u][r][2] + v[u][r][3]);
-    const float mu = row_sum<G, WG>(s, scratch, turn) * inv_d;
-    float q = 0.0f;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int c = (r * G + lane) * 4;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[u][r][i] -= mu;
-        if ((r + 1) * G * 4 > LO && c + i >= p.D) v[u][r][i] = 0.0f;
-        q = __builtin_fmaf(v[u][r][i], v[u][r][i], q);
-      }
+    for (int u = 0; u < RU; ++u) {
+      const int64_t row = row0 + u * GROUPS;  // past the end: the last row again, not stored
+      load_row<G, R, LO, true>(x + (row < p.M ? row : p.M - 1) * p.ldx, lane, p.D, 0.0f, v[u]);
     }
-    const float rs = 1.0f / sqrtf(row_sum<G, WG>(q, scratch, turn) * inv_d + p.eps);
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int u = 0; u < RU; ++u) {
+      const int64_t row = row0 + u * GROUPS;
+      float s = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[u][r][i] = __builtin_fmaf(v[u][r][i] * rs, w[r][i], b[r][i]);
-    if (row < p.M) {
-      if (p.stats && lane == 0) p.stats[row] = make_float2(mu, rs);
-      store_row<G, R, LO, true>(y + row * p.ldy, lane, p.D, v[u]);
+      for (int r = 0; r < R; ++r) s += (v[u][r][0] + v[u][r][1]) + (v[u][r][2] + v[u][r][3]);
+      const float mu = row_sum<G, WG>(s, scratch, turn) * inv_d;
+      float q = 0.0f;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int c = (r * G + lane) * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[u][r][i] -= mu;
+          if ((r + 1) * G * 4 > LO && c + i >= p.D) v[u][r][i] = 0.0f;
+          q = __builtin_fmaf(v[u][r][i], v[u][r][i], q);
+        }
+      }
+      const float rs = 1.0f / sqrtf(row_sum<G, WG>(q, scratch, turn) * inv_d + p.eps);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[u][r][i] = __builtin_fmaf(v[u][r][i] * rs, w[r][i], b[r][i]);
+      if (row < p.M) {
+        if (p.stats && lane == 0) p.stats[row] = make_float2(mu, rs);
+        store_row<G, R, LO, true>(y + row * p.ldy, lane, p.D, v[u]);
+      }
     }
   }
 }
@@ -322,8 +327,9 @@ void launch_fwd(const FwdArgs& a, hipStream_t st) {
   with_form(a.D, [&](auto form) {
     using F = decltype(form);
     constexpr int RU = F::r == 1 ? 2 : 1, rows = threads_of(F::g) / F::g * RU;
+    const int64_t groups = (a.M + rows - 1) / rows;
     ln_fwd_kernel<T, F::g, F::r, F::lo, RU>
-        <<<static_cast<unsigned>((a.M + rows - 1) / rows), threads_of(F::g), 0, st>>>(a);
+        <<<static_cast<unsigned>(groups < kMaxGroups ? groups : kMaxGroups), threads_of(F::g), 0, st>>>(a);
   });
 }
 
@@ -334,6 +340,8 @@ int64_t bwd_rows(int64_t M, int64_t D) {
   with_form(static_cast<int>(D), [&](auto form) { groups = threads_of(decltype(form)::g) / decltype(form)::g; });
   int64_t rows = (M + 511) / 512;
   rows = rows < 64 ? rows : 64;
+  const int64_t least = (M + kMaxParts - 1) / kMaxParts;
+  rows = rows > least ? rows : least;
   return (rows + groups - 1) / groups * groups;
 }
 int64_t bwd_parts(int64_t M, int64_t D) { return (M + bwd_rows(M, D) - 1) / bwd_rows(M, D); }

@@ -688,3 +688,56 @@ def test_offsets_past_32_bits(dev):
 
 def test_library_was_used(dev):
     assert nv.lib().spmi_version() >= 100
+
+
+def test_more_rows_than_a_grid_has_waves(dev):
+    """2^24 rows and some: the launches are bounded, the kernels go on."""
+    m = (1 << 24) + 77
+    x = torch.zeros(m, 4, dtype=BF16, device=dev)
+    x[-100:] = rand(100, 4, dtype=BF16)
+    q, scale = ops.quantize_rows_int8(x)
+    want_q, want_s = quantized(x[-100:])
+    assert torch.equal(q[-100:].double().cpu(), want_q) and int(q[:-100].count_nonzero()) == 0
+    within(scale[-100:], want_s, U * want_s)
+    y = ops.layer_norm(x)
+    assert torch.equal(y[-100:], ops.layer_norm(x[-100:].clone())) and int(y[:-100].count_nonzero()) == 0
+
+
+def test_empty_problems(dev):
+    h, last = ops.gated_scan(torch.zeros(5, 0, 8, device=dev))
+    assert h.shape == (5, 0, 4) and last.shape == (0, 4)
+    gates = torch.zeros(0, 3, 8, device=dev, requires_grad=True)
+    h0 = rand(3, 4).requires_grad_()
+    h, last = ops.gated_scan(gates, h0)
+    (g,) = torch.autograd.grad(last, h0, rand(3, 4, seed=1))
+    assert torch.equal(last, h0) and torch.equal(g, rand(3, 4, seed=1))
+    x, w = torch.zeros(0, 8, device=dev, requires_grad=True), torch.ones(8, device=dev, requires_grad=True)
+    gx, gw = torch.autograd.grad(ops.layer_norm(x, w).sum(), (x, w))
+    assert gx.shape == (0, 8) and bool((gw == 0).all())
+    mem = torch.zeros(0, 4, device=dev)
+    assert bool(ops.gated_step(torch.zeros(2, 8, device=dev), mem, torch.zeros(2, dtype=torch.int64, device=dev)).isnan().all())
+    assert ops.quantize_rows_int8(torch.zeros(0, 8, device=dev))[0].shape == (0, 8)
+
+
+def test_inference_mode(dev):
+    mem = rand(6, 8)
+    want = ops.gated_step(rand(6, 16), mem.clone())
+    with torch.inference_mode():
+        inside = mem.clone()
+        assert torch.equal(ops.gated_step(rand(6, 16), inside), want) and torch.equal(inside, want)
+        assert torch.equal(ops.gated_step(rand(6, 16), mem), want) and torch.equal(mem, want)
+        wq, ws = weight8(5, 8)
+        assert ops.linear_int8(ops.layer_norm(mem), wq, ws).shape == (6, 5)
+
+
+def test_a_backward_pass_runs_twice_and_sees_changed_inputs(dev):
+    gates, h0 = rand(40, 3, 16).requires_grad_(), rand(3, 8, seed=1).requires_grad_()
+    h, last = ops.gated_scan(gates, h0)
+    g = rand(40, 3, 8, seed=2)
+    first = torch.autograd.grad(h, (gates, h0), g, retain_graph=True)
+    second = torch.autograd.grad(h, (gates, h0), g, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    with torch.no_grad():
+        h.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified"):
+        torch.autograd.grad(h, (gates, h0), g)
