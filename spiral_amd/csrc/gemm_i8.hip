@@ -68,61 +68,61 @@ __device__ __forceinline__ unsigned pack4(const float (&v)[4], float inv) {
 }
 
 // q [M, width] (width >= K, zero past K) and the rows' scales.  A wave per row, which it keeps in
-// registers (R pieces of 256 values); R = 0: rows of any length, read twice.
+// registers: R pieces of 64 lanes times 16 bytes (four values of float32, eight of bfloat16).  R = 0:
+// rows of any length, read twice.
 template <typename T, int R>
 __global__ __launch_bounds__(kThreads) void quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t M, int K,
                                                             int8_t* __restrict__ q, int64_t ldq, int width,
                                                             float* __restrict__ scale) {
+  constexpr int V = 16 / sizeof(T) / 4;  // fours of a lane
+  constexpr int PIECE = 256 * V;
   const int lane = threadIdx.x & 63;
   for (int64_t row = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 6; row < M;
        row += (static_cast<int64_t>(gridDim.x) * kThreads) >> 6) {
     const T* const src = x + row * ldx;
     int8_t* const dst = q + row * ldq;
     unsigned top = 0;
-    float v[R > 0 ? R : 1][4];
-    if constexpr (R > 0) {
+    const auto fetch = [&](int c, float (&v)[V][4]) {
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const int c = r * 256 + lane * 4;
+      for (int u = 0; u < V; ++u) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[r][i] = 0.0f;
-        if (c < K) load4_upto<true>(src + c, K - c, 0.0f, v[r]);
+        for (int i = 0; i < 4; ++i) v[u][i] = 0.0f;
+        if (c + 4 * u < K) load4_upto<true>(src + c + 4 * u, K - c - 4 * u, 0.0f, v[u]);
+        top = top_of(top, v[u]);
       }
-#pragma unroll
-      for (int r = 0; r < R; ++r) top = top_of(top, v[r]);
-    } else {
-#pragma unroll 4
-      for (int c = lane * 4; c < K; c += 256) {
-        load4_upto(src + c, K - c, 0.0f, v[0]);
-        top = top_of(top, v[0]);
-      }
-    }
-    top = group_top<64>(top);
+    };
     float inv, s;
-    row_scale(top, inv, s);
-    if (lane == 0) scale[row] = s;
-    const auto put = [&](int c, const float (&t)[4]) {
-      const unsigned w = pack4(t, inv);
-      if (c + 4 <= width) {
-        __builtin_memcpy(dst + c, &w, 4);
+    const auto put = [&](int c, const float (&v)[V][4]) {
+      unsigned w[V];
+#pragma unroll
+      for (int u = 0; u < V; ++u) w[u] = pack4(v[u], inv);
+      if (c + 4 * V <= width) {
+        __builtin_memcpy(dst + c, w, 4 * V);
       } else {
 #pragma unroll
-        for (int i = 0; i < 3; ++i)
-          if (c + i < width) dst[c + i] = static_cast<int8_t>(w >> (8 * i));
+        for (int i = 0; i < 4 * V - 1; ++i)
+          if (c + i < width) dst[c + i] = static_cast<int8_t>(w[i / 4] >> (8 * (i & 3)));
       }
     };
     if constexpr (R > 0) {
+      float v[R][V][4];
 #pragma unroll
-      for (int r = 0; r < R; ++r) put(r * 256 + lane * 4, v[r]);
+      for (int r = 0; r < R; ++r) fetch(r * PIECE + lane * 4 * V, v[r]);
+      row_scale(group_top<64>(top), inv, s);
+#pragma unroll
+      for (int r = 0; r < R; ++r) put(r * PIECE + lane * 4 * V, v[r]);
     } else {
+      float v[V][4];
 #pragma unroll 4
-      for (int c = lane * 4; c < width; c += 256) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[0][i] = 0.0f;
-        if (c < K) load4_upto(src + c, K - c, 0.0f, v[0]);
-        put(c, v[0]);
+      for (int c = lane * 4 * V; c < K; c += PIECE) fetch(c, v);
+      row_scale(group_top<64>(top), inv, s);
+#pragma unroll 4
+      for (int c = lane * 4 * V; c < width; c += PIECE) {
+        fetch(c, v);
+        put(c, v);
       }
     }
+    if (lane == 0) scale[row] = s;
   }
 }
 
@@ -844,11 +844,12 @@ void launch_quantize(const void* x, int64_t ldx, int64_t M, int64_t K, int8_t* q
     quantize_kernel<T, decltype(r)::value><<<static_cast<unsigned>((M + 3) / 4 < kMaxGroups ? (M + 3) / 4 : kMaxGroups), kThreads, 0, st>>>(
         static_cast<const T*>(x), ldx, M, static_cast<int>(K), q, ldq, static_cast<int>(width), scale);
   };
-  if (width <= 256) go(std::integral_constant<int, 1>{});
-  else if (width <= 512) go(std::integral_constant<int, 2>{});
-  else if (width <= 1024) go(std::integral_constant<int, 4>{});
-  else if (width <= 2048) go(std::integral_constant<int, 8>{});
-  else if (width <= 4096) go(std::integral_constant<int, 16>{});
+  const int64_t pieces = (width * static_cast<int64_t>(sizeof(T)) + 1023) / 1024;
+  if (pieces <= 1) go(std::integral_constant<int, 1>{});
+  else if (pieces <= 2) go(std::integral_constant<int, 2>{});
+  else if (pieces <= 4) go(std::integral_constant<int, 4>{});
+  else if (pieces <= 8) go(std::integral_constant<int, 8>{});
+  else if (sizeof(T) == 4 && pieces <= 16) go(std::integral_constant<int, sizeof(T) == 4 ? 16 : 0>{});
   else go(std::integral_constant<int, 0>{});
 }
 void launch_quantize(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, int8_t* q, int64_t ldq,

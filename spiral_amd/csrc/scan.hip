@@ -89,16 +89,20 @@ __device__ __forceinline__ void gate_pair(float z, float& a, float& rest) {
   rest = z >= 0.0f ? small : big;
 }
 
-// What a thread works on: four units of one node.
+// What a thread works on: four units of one node.  The last four of a row whose length is no multiple
+// of four reach back into the units of the thread before: both compute the same bits from the same
+// inputs and write them to the same places, and no access has an end to look at.  (Rows of fewer than
+// four units do: `left`, the same for all.)
 struct Place {
   bool there;
   int64_t n;
-  int c, left;  // first unit, units from it to the end of the row
+  int c, left;
   __device__ Place(const ScanArgs& p, int64_t lane) {
     there = lane < p.N * p.Hq;
     n = there ? lane / p.Hq : 0;
     c = there ? static_cast<int>(lane - n * p.Hq) * 4 : 0;
-    left = p.H - c;
+    if (p.H >= 4 && c > p.H - 4) c = p.H - 4;
+    left = p.H < 4 ? p.H : 4;
   }
 };
 
