@@ -26,6 +26,8 @@
 // is stored.  Steps where a node is not active pass the state (and its gradient) on unchanged;
 // what stands in the gates there is loaded but never used.
 
+#include <type_traits>
+
 #include "lanes.h"
 
 namespace {
@@ -33,12 +35,14 @@ namespace {
 using namespace spmi;
 
 constexpr int kThreads = 256;
-// Steps a thread holds in registers, as one of the strands and walking.  Walking, fewer steps leave room
-// for more waves, which pays for bfloat16, whose loads are half as wide: 249 us with 2 steps against
-// 284 with 4 forward (32 x 50000 x 128), 957 against 1371 with the backward pass (2 steps, four waves
-// to a SIMD); float32 is level forward (480, 482) and a little better with 4 backward.
-constexpr int kFwdSteps = 4;
-constexpr int kFwdWalkSteps = 2;
+// Steps a thread holds in registers.  Walking, the loads of the next steps are sent before the stores of
+// the present ones: 32 x 50000 x 128 takes 481 us forward and 1388 trained in float32, 244 and 690 in
+// bfloat16 (without: 494, 1431, 246, 704; with 2 steps forward 488, 1410).  As one of the strands, other
+// waves cover the wait better than registers do (four waves to a SIMD: 1185 x 2255 x 30 trained in
+// bfloat16 539 us, with six 765), and more steps pay less than they cost: 65536 x 1 x 128 42 us with 2
+// forward, 49 with 4; 1601 x 717 x 64 trained in float32 692 with 2 backward, 819 with 4.
+constexpr int kFwdSteps = 2;
+constexpr int kFwdWalkSteps = 4;
 constexpr int kBwdSteps = 2;
 template <typename T>
 constexpr int kBwdWalkSteps = sizeof(T) == 4 ? 4 : 2;
@@ -48,7 +52,11 @@ constexpr int kStrands = kThreads / kLanes;
 constexpr int64_t kManyLanes = 65536;
 // Up to this many steps there is nothing to share among the strands.
 constexpr int64_t kFewSteps = 16;
-constexpr int64_t kTargetGroups = 2048;  // workgroups wanted before the steps are split further
+// Workgroups from which the steps are not split: two per CU (852 x 221 x 448 in bfloat16, 774 workgroups, takes
+// 139 us unsplit and 188 in two, which read the gates twice).  Below, as many splits as make kTargetGroups
+// (1601 x 717 x 64, 359 workgroups, trained in bfloat16 406 us in five, 478 in two).
+constexpr int64_t kEnoughGroups = 512;
+constexpr int64_t kTargetGroups = 2048;
 constexpr int64_t kMaxSplits = 512;
 
 struct ScanArgs {
@@ -106,8 +114,42 @@ struct Place {
   }
 };
 
+// Four values as they are stored.  The loads of several steps are issued without a branch or a conversion
+// between them, and widened when they are used: with either in between, each load is waited for before
+// the next is sent.  TINY: rows of fewer than four units.
+using f32x4_held = float __attribute__((ext_vector_type(4)));
+using u16x4_held = unsigned short __attribute__((ext_vector_type(4)));
+template <typename T> struct Held;
+template <> struct Held<float> { using type = f32x4_held; using any = f32x4_any; };
+template <> struct Held<bf16> { using type = u16x4_held; using any = u16x4_any; };
+template <typename T>
+using held = typename Held<T>::type;
+
+template <bool STREAM, bool TINY, typename T>
+__device__ __forceinline__ held<T> take(const T* p, int left) {
+  held<T> v;
+  if constexpr (TINY) {
+    const auto* q = reinterpret_cast<const std::conditional_t<sizeof(T) == 4, float, unsigned short>*>(p);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = q[k < left ? k : left - 1];
+  } else {
+    const auto* q = reinterpret_cast<const typename Held<T>::any*>(p);
+    v = STREAM ? __builtin_nontemporal_load(q) : *q;
+  }
+  return v;
+}
+__device__ __forceinline__ float widen(float v) { return v; }
+__device__ __forceinline__ float widen(unsigned short v) {
+  return __builtin_bit_cast(float, static_cast<unsigned>(v) << 16);
+}
+template <bool TINY, typename T>
+__device__ __forceinline__ void put(T* p, int left, const float (&v)[4]) {
+  if constexpr (TINY) store4_upto(p, left, v);
+  else store4<true>(p, v);
+}
+
 // Forward.  C lanes x S strands; MAPS: only the map of the split is wanted.
-template <typename T, int C, int S, bool MAPS>
+template <typename T, int C, int S, bool MAPS, bool TINY>
 __global__ __launch_bounds__(kThreads, S > 1 ? 4 : 1) void scan_fwd_kernel(ScanArgs p) {
   constexpr int L = S == 1 ? kFwdWalkSteps : kFwdSteps;
   constexpr bool STREAM = S == 1;  // a split sequence is read twice, the second time from the caches
@@ -125,32 +167,38 @@ __global__ __launch_bounds__(kThreads, S > 1 ? 4 : 1) void scan_fwd_kernel(ScanA
 
   // Loads without a condition around them, so that those of all steps are in flight together: steps past
   // the end read the last one again, lanes past the end the first node's.  `on` says what counts.
-  float a[L][4], b[L][4];
-  bool on[L];
+  held<T> raw_z[L], raw_c[L];
+  unsigned act[L];
   auto fetch = [&](int64_t t0) {
-    unsigned act[L];
 #pragma unroll
     for (int i = 0; i < L; ++i) {
       int64_t t = t0 + strand * L + i;
       t = t < t_end ? t : t_end - 1;
-      act[i] = active ? active[t * p.active_t] : 1u;
-      load4_upto<STREAM>(gates + t * p.gates_t, at.left, 0.0f, a[i]);
-      load4_upto<STREAM>(gates + t * p.gates_t + p.H, at.left, 0.0f, b[i]);
+      raw_z[i] = take<STREAM, TINY>(gates + t * p.gates_t, at.left);
+      raw_c[i] = take<STREAM, TINY>(gates + t * p.gates_t + p.H, at.left);
     }
+    if (active) {
 #pragma unroll
-    for (int i = 0; i < L; ++i) on[i] = t0 + strand * L + i < t_end && act[i] != 0;
+      for (int i = 0; i < L; ++i) {
+        int64_t t = t0 + strand * L + i;
+        act[i] = active[(t < t_end ? t : t_end - 1) * p.active_t];
+      }
+    }
   };
+  float a[L][4], b[L][4];
   // z, c -> the step's map (a, (1 - a) c)
-  auto to_maps = [&]() {
+  auto to_maps = [&](int64_t t0) {
 #pragma unroll
-    for (int i = 0; i < L; ++i)
+    for (int i = 0; i < L; ++i) {
+      const bool on = t0 + strand * L + i < t_end && (!active || act[i] != 0);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        float keep, rest;
-        gate_pair(a[i][k], keep, rest);
-        b[i][k] = on[i] ? rest * b[i][k] : 0.0f;
-        a[i][k] = on[i] ? keep : 1.0f;
+        // chosen before the arithmetic, not after: there is no branch around it then
+        float rest;
+        gate_pair(on ? widen(raw_z[i][k]) : __builtin_inff(), a[i][k], rest);
+        b[i][k] = rest * (on ? widen(raw_c[i][k]) : 0.0f);
       }
+    }
   };
 
   if (t_begin < t_end) fetch(t_begin);
@@ -192,8 +240,9 @@ __global__ __launch_bounds__(kThreads, S > 1 ? 4 : 1) void scan_fwd_kernel(ScanA
 
   int turn = 0;
   for (int64_t t0 = t_begin; t0 < t_end; t0 += S * L) {
-    if (t0 != t_begin) fetch(t0);
-    to_maps();
+    if (S > 1 && t0 != t_begin) fetch(t0);
+    to_maps(t0);
+    if (S == 1 && t0 + L < t_end) fetch(t0 + L);  // the next steps' loads, before this one's stores
     float start[4];
     if constexpr (S > 1) {
       float P[4] = {1.0f, 1.0f, 1.0f, 1.0f}, Q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -232,7 +281,7 @@ __global__ __launch_bounds__(kThreads, S > 1 ? 4 : 1) void scan_fwd_kernel(ScanA
         const int64_t t = t0 + strand * L + i;
 #pragma unroll
         for (int k = 0; k < 4; ++k) start[k] = __builtin_fmaf(a[i][k], start[k], b[i][k]);
-        if (at.there && t < t_end) store4_upto<true>(out + t * p.h_t, at.left, start);
+        if (at.there && t < t_end) put<TINY>(out + t * p.h_t, at.left, start);
       }
       if constexpr (S == 1) {
 #pragma unroll
@@ -255,7 +304,7 @@ __global__ __launch_bounds__(kThreads, S > 1 ? 4 : 1) void scan_fwd_kernel(ScanA
 
 // Backward, from the last step down: strand 0 has the latest steps of a tile, split 0 the latest
 // steps of all.
-template <typename T, int C, int S, bool MAPS>
+template <typename T, int C, int S, bool MAPS, bool TINY>
 __global__ __launch_bounds__(kThreads, S > 1 || sizeof(T) == 2 ? 4 : 1) void scan_bwd_kernel(ScanArgs p) {
   constexpr int L = S == 1 ? kBwdWalkSteps<T> : kBwdSteps;
   constexpr bool STREAM = S == 1;
@@ -274,43 +323,33 @@ __global__ __launch_bounds__(kThreads, S > 1 || sizeof(T) == 2 ? 4 : 1) void sca
   const T* h = static_cast<const T*>(p.h) + at.n * p.h_n + at.c;
   const uint8_t* active = p.active ? p.active + at.n * p.active_n : nullptr;
 
-  float z[L][4], c[L][4], gv[L][4], hp[L][4];
-  bool on[L];
+  held<T> raw_z[L], raw_c[L], raw_g[L], raw_h[L];
+  unsigned act[L];
   auto fetch = [&](int64_t u0) {
-    unsigned act[L];
 #pragma unroll
     for (int i = 0; i < L; ++i) {
       int64_t u = u0 + strand * L + i;
       u = u < u_end ? u : u_end - 1;
       const int64_t t = p.T - 1 - u;
-      act[i] = active ? active[t * p.active_t] : 1u;
-      load4_upto<STREAM>(gates + t * p.gates_t, at.left, 0.0f, z[i]);
-      if (p.g) {
-        load4_upto<STREAM>(g + t * p.g_t, at.left, 0.0f, gv[i]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) gv[i][k] = 0.0f;
-      }
+      raw_z[i] = take<STREAM, TINY>(gates + t * p.gates_t, at.left);
       if constexpr (!MAPS) {
-        load4_upto<STREAM>(gates + t * p.gates_t + p.H, at.left, 0.0f, c[i]);
+        raw_c[i] = take<STREAM, TINY>(gates + t * p.gates_t + p.H, at.left);
         // the state before the step; before the first one it is h0, put in below
-        if (p.T > 1) load4_upto<STREAM>(h + (t > 0 ? t - 1 : 0) * p.h_t, at.left, 0.0f, hp[i]);
+        raw_h[i] = take<STREAM, TINY>(h + (t > 0 ? t - 1 : 0) * p.h_t, at.left);
       }
     }
+    if (p.g) {
 #pragma unroll
-    for (int i = 0; i < L; ++i) {
-      const int64_t u = u0 + strand * L + i;
-      on[i] = u < u_end && act[i] != 0;
-      if constexpr (!MAPS) {
-        if (u == p.T - 1) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) hp[i][k] = 0.0f;
-          if (p.h0) load4_upto(p.h0 + at.n * p.h0_n + at.c, at.left, 0.0f, hp[i]);
-        }
+      for (int i = 0; i < L; ++i) {
+        const int64_t u = u0 + strand * L + i;
+        raw_g[i] = take<STREAM, TINY>(g + (p.T - 1 - (u < u_end ? u : u_end - 1)) * p.g_t, at.left);
       }
-      if (u >= u_end) {
+    }
+    if (active) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) gv[i][k] = 0.0f;  // a step that is not there passes e on as it is
+      for (int i = 0; i < L; ++i) {
+        const int64_t u = u0 + strand * L + i;
+        act[i] = active[(p.T - 1 - (u < u_end ? u : u_end - 1)) * p.active_t];
       }
     }
   };
@@ -351,15 +390,30 @@ __global__ __launch_bounds__(kThreads, S > 1 || sizeof(T) == 2 ? 4 : 1) void sca
 
   int turn = 0;
   for (int64_t u0 = u_begin; u0 < u_end; u0 += S * L) {
-    if (u0 != u_begin) fetch(u0);
-    float a[L][4], rest[L][4];
+    if (S > 1 && u0 != u_begin) fetch(u0);
+    float a[L][4], rest[L][4], gv[L][4], away[L][4];  // away: the state before the step, less c
+    bool on[L];
 #pragma unroll
-    for (int i = 0; i < L; ++i)
+    for (int i = 0; i < L; ++i) {
+      const int64_t u = u0 + strand * L + i;
+      on[i] = u < u_end && (!active || act[i] != 0);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        gate_pair(z[i][k], a[i][k], rest[i][k]);
-        if (!on[i]) a[i][k] = 1.0f;
+        gate_pair(on[i] ? widen(raw_z[i][k]) : __builtin_inff(), a[i][k], rest[i][k]);  // 1, 0 for a step passed over
+        // a step that is not there passes e on as it is
+        gv[i][k] = p.g && u < u_end ? widen(raw_g[i][k]) : 0.0f;
+        if constexpr (!MAPS) away[i][k] = widen(raw_h[i][k]) - widen(raw_c[i][k]);
       }
+      if constexpr (!MAPS) {
+        if (u == p.T - 1) {
+          float before[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          if (p.h0) load4_upto(p.h0 + at.n * p.h0_n + at.c, at.left, 0.0f, before);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) away[i][k] = before[k] - widen(raw_c[i][k]);
+        }
+      }
+    }
+    if (S == 1 && u0 + L < u_end) fetch(u0 + L);
     float start[4];
     if constexpr (S > 1) {
       float P[4] = {1.0f, 1.0f, 1.0f, 1.0f}, Q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -401,12 +455,12 @@ __global__ __launch_bounds__(kThreads, S > 1 || sizeof(T) == 2 ? 4 : 1) void sca
         for (int k = 0; k < 4; ++k) {
           const float d = start[k] + gv[i][k];
           dc[k] = on[i] ? d * rest[i][k] : 0.0f;
-          dz[k] = on[i] ? d * (hp[i][k] - c[i][k]) * (a[i][k] * rest[i][k]) : 0.0f;
+          dz[k] = on[i] ? d * away[i][k] * (a[i][k] * rest[i][k]) : 0.0f;
           start[k] = a[i][k] * d;
         }
         if (p.dgates && at.there && u < u_end) {
-          store4_upto<true>(out + t * p.dg_t, at.left, dz);
-          store4_upto<true>(out + t * p.dg_t + p.H, at.left, dc);
+          put<TINY>(out + t * p.dg_t, at.left, dz);
+          put<TINY>(out + t * p.dg_t + p.H, at.left, dc);
         }
       }
       if constexpr (S == 1) {
@@ -440,8 +494,8 @@ Plan plan_for(int64_t T, int64_t N, int64_t H, int steps) {
   const int64_t tile = static_cast<int64_t>(kStrands) * steps;
   const int64_t tiles = (T + tile - 1) / tile;
   const int64_t groups = (lanes + kLanes - 1) / kLanes;
-  int64_t splits = kTargetGroups / groups;
-  splits = splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits;
+  int64_t splits = groups >= kEnoughGroups ? 1 : kTargetGroups / groups;
+  splits = splits > kMaxSplits ? kMaxSplits : splits;
   splits = splits < tiles ? splits : tiles;
   const int64_t per = (tiles + splits - 1) / splits * tile;
   return {false, static_cast<int>((T + per - 1) / per), per};
@@ -451,29 +505,29 @@ size_t maps_bytes(int64_t T, int64_t N, int64_t H, int steps) {
   return q.splits > 1 ? static_cast<size_t>(q.splits) * 2 * N * ((H + 3) / 4) * 4 * sizeof(float) : 0;
 }
 
-template <typename T>
-void launch_fwd(ScanArgs a, const Plan& q, hipStream_t st) {
+template <typename T, bool TINY>
+void launch_fwd(const ScanArgs& a, const Plan& q, hipStream_t st) {
   const int64_t lanes = a.N * a.Hq;
   if (q.walk) {
-    scan_fwd_kernel<T, kThreads, 1, false><<<(lanes + kThreads - 1) / kThreads, kThreads, 0, st>>>(a);
+    scan_fwd_kernel<T, kThreads, 1, false, TINY><<<(lanes + kThreads - 1) / kThreads, kThreads, 0, st>>>(a);
     return;
   }
   const unsigned groups = static_cast<unsigned>((lanes + kLanes - 1) / kLanes);
   if (q.splits > 1)  // the last split's map starts nothing
-    scan_fwd_kernel<T, kLanes, kStrands, true><<<dim3(groups, q.splits - 1), kThreads, 0, st>>>(a);
-  scan_fwd_kernel<T, kLanes, kStrands, false><<<dim3(groups, q.splits), kThreads, 0, st>>>(a);
+    scan_fwd_kernel<T, kLanes, kStrands, true, TINY><<<dim3(groups, q.splits - 1), kThreads, 0, st>>>(a);
+  scan_fwd_kernel<T, kLanes, kStrands, false, TINY><<<dim3(groups, q.splits), kThreads, 0, st>>>(a);
 }
-template <typename T>
-void launch_bwd(ScanArgs a, const Plan& q, hipStream_t st) {
+template <typename T, bool TINY>
+void launch_bwd(const ScanArgs& a, const Plan& q, hipStream_t st) {
   const int64_t lanes = a.N * a.Hq;
   if (q.walk) {
-    scan_bwd_kernel<T, kThreads, 1, false><<<(lanes + kThreads - 1) / kThreads, kThreads, 0, st>>>(a);
+    scan_bwd_kernel<T, kThreads, 1, false, TINY><<<(lanes + kThreads - 1) / kThreads, kThreads, 0, st>>>(a);
     return;
   }
   const unsigned groups = static_cast<unsigned>((lanes + kLanes - 1) / kLanes);
   if (q.splits > 1)
-    scan_bwd_kernel<T, kLanes, kStrands, true><<<dim3(groups, q.splits - 1), kThreads, 0, st>>>(a);
-  scan_bwd_kernel<T, kLanes, kStrands, false><<<dim3(groups, q.splits), kThreads, 0, st>>>(a);
+    scan_bwd_kernel<T, kLanes, kStrands, true, TINY><<<dim3(groups, q.splits - 1), kThreads, 0, st>>>(a);
+  scan_bwd_kernel<T, kLanes, kStrands, false, TINY><<<dim3(groups, q.splits), kThreads, 0, st>>>(a);
 }
 
 int check_sizes(const char* what, int dtype, int64_t T, int64_t N, int64_t H) {
@@ -595,8 +649,9 @@ int spmi_gated_scan_fwd(const void* gates, int dtype, int64_t gates_t, int64_t g
   a.h = h; a.h_t = h_t; a.h_n = h_n; a.last = last;
   a.T = T; a.N = N; a.H = static_cast<int>(H); a.Hq = static_cast<int>((H + 3) / 4);
   a.per_split = q.per_split; a.splits = q.splits; a.maps = static_cast<float*>(ws);
-  if (dtype == SPMI_DTYPE_F32) launch_fwd<float>(a, q, as_stream(stream));
-  else launch_fwd<bf16>(a, q, as_stream(stream));
+  const bool tiny = H < 4;
+  if (dtype == SPMI_DTYPE_F32) (tiny ? launch_fwd<float, true> : launch_fwd<float, false>)(a, q, as_stream(stream));
+  else (tiny ? launch_fwd<bf16, true> : launch_fwd<bf16, false>)(a, q, as_stream(stream));
   SPMI_CHECK_LAUNCH("spmi_gated_scan_fwd");
   return SPMI_OK;
 }
@@ -619,12 +674,16 @@ int spmi_gated_scan_bwd(const void* gates, int dtype, int64_t gates_t, int64_t g
   a.h0 = h0; a.h0_n = h0_n;
   a.active = active; a.active_t = active_t; a.active_n = active_n;
   a.h = const_cast<void*>(h); a.h_t = h_t; a.h_n = h_n;
+  if (T == 1) {  // there may be no h: what is read in place of the states before the first step is not used
+    a.h = const_cast<void*>(gates); a.h_t = gates_t; a.h_n = gates_n;
+  }
   a.g = g; a.g_t = g_t; a.g_n = g_n; a.g_last = g_last; a.gl_n = gl_n;
   a.dgates = dgates; a.dg_t = dg_t; a.dg_n = dg_n; a.dh0 = dh0;
   a.T = T; a.N = N; a.H = static_cast<int>(H); a.Hq = static_cast<int>((H + 3) / 4);
   a.per_split = q.per_split; a.splits = q.splits; a.maps = static_cast<float*>(ws);
-  if (dtype == SPMI_DTYPE_F32) launch_bwd<float>(a, q, as_stream(stream));
-  else launch_bwd<bf16>(a, q, as_stream(stream));
+  const bool tiny = H < 4;
+  if (dtype == SPMI_DTYPE_F32) (tiny ? launch_bwd<float, true> : launch_bwd<float, false>)(a, q, as_stream(stream));
+  else (tiny ? launch_bwd<bf16, true> : launch_bwd<bf16, false>)(a, q, as_stream(stream));
   SPMI_CHECK_LAUNCH("spmi_gated_scan_bwd");
   return SPMI_OK;
 }
