@@ -82,12 +82,14 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const T* __restrict_
     const T* const src = x + row * ldx;
     int8_t* const dst = q + row * ldq;
     unsigned top = 0;
-    const auto fetch = [&](int c, float (&v)[V][4]) {
+    const auto fetch = [&](int c, held<T> (&raw)[V]) {
+#pragma unroll
+      for (int u = 0; u < V; ++u) raw[u] = hold_row<true>(src, c + 4 * u, K);
+    };
+    const auto look = [&](int c, const held<T> (&raw)[V], float (&v)[V][4]) {
 #pragma unroll
       for (int u = 0; u < V; ++u) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[u][i] = 0.0f;
-        if (c + 4 * u < K) load4_upto<true>(src + c + 4 * u, K - c - 4 * u, 0.0f, v[u]);
+        widen_row<T>(raw[u], c + 4 * u, K, v[u]);
         top = top_of(top, v[u]);
       }
     };
@@ -105,20 +107,28 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const T* __restrict_
       }
     };
     if constexpr (R > 0) {
+      held<T> raw[R][V];
       float v[R][V][4];
 #pragma unroll
-      for (int r = 0; r < R; ++r) fetch(r * PIECE + lane * 4 * V, v[r]);
+      for (int r = 0; r < R; ++r) fetch(r * PIECE + lane * 4 * V, raw[r]);
+#pragma unroll
+      for (int r = 0; r < R; ++r) look(r * PIECE + lane * 4 * V, raw[r], v[r]);
       row_scale(group_top<64>(top), inv, s);
 #pragma unroll
       for (int r = 0; r < R; ++r) put(r * PIECE + lane * 4 * V, v[r]);
     } else {
+      held<T> raw[V];
       float v[V][4];
 #pragma unroll 4
-      for (int c = lane * 4 * V; c < K; c += PIECE) fetch(c, v);
+      for (int c = lane * 4 * V; c < K; c += PIECE) {
+        fetch(c, raw);
+        look(c, raw, v);
+      }
       row_scale(group_top<64>(top), inv, s);
 #pragma unroll 4
       for (int c = lane * 4 * V; c < width; c += PIECE) {
-        fetch(c, v);
+        fetch(c, raw);
+        look(c, raw, v);
         put(c, v);
       }
     }
@@ -671,11 +681,15 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_i8_kernel(FewArgs p) {
     for (int r0 = 0; r0 < p.M; r0 += 4) {
       unsigned top[4] = {0, 0, 0, 0};
       for (int c = tid * 4; c < p.K; c += NW * 256) {
-        float v[4][4];
+        held<T> raw[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) load4_upto(x + (r0 + j < p.M ? r0 + j : r0) * p.ldx + c, p.K - c, 0.0f, v[j]);
+        for (int j = 0; j < 4; ++j) raw[j] = hold_row<false>(x + (r0 + j < p.M ? r0 + j : r0) * p.ldx, c, p.K);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) top[j] = top_of(top[j], v[j]);
+        for (int j = 0; j < 4; ++j) {
+          float v[4];
+          widen_row<T>(raw[j], c, p.K, v);
+          top[j] = top_of(top[j], v);
+        }
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -697,13 +711,15 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_i8_kernel(FewArgs p) {
         if (tid == 0) row_scale_of[r] = s;
       }
       for (int c = tid * 4; c < KP; c += NW * 256) {
-        float v[4][4] = {};
+        held<T> raw[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (c < p.K) load4_upto(x + (r0 + j < p.M ? r0 + j : r0) * p.ldx + c, p.K - c, 0.0f, v[j]);
+        for (int j = 0; j < 4; ++j) raw[j] = hold_row<false>(x + (r0 + j < p.M ? r0 + j : r0) * p.ldx, c, p.K);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (r0 + j < p.M) *reinterpret_cast<unsigned*>(q + (r0 + j) * SK + c) = pack4(v[j], inv[j]);
+        for (int j = 0; j < 4; ++j) {
+          float v[4];
+          widen_row<T>(raw[j], c, p.K, v);
+          if (r0 + j < p.M) *reinterpret_cast<unsigned*>(q + (r0 + j) * SK + c) = pack4(v, inv[j]);
+        }
       }
     }
     __syncthreads();

@@ -2,6 +2,8 @@
 // float or bfloat16 rows as float, and reductions over neighbouring lanes.
 #pragma once
 
+#include <type_traits>
+
 #include "common.h"
 
 namespace spmi {
@@ -50,7 +52,62 @@ __device__ __forceinline__ void store4(bf16* p, const float (&v)[4]) {
   else *q = t;
 }
 
-// The same for the last values of a row: `left` >= 1 of them exist, the others read as `fill`.
+// Four values as they are stored.  Loads that should be in flight together are issued as these, without a
+// branch or a conversion between them, and widened where they are used: with either in between, each
+// load is waited for before the next is sent.
+template <typename T> struct Held;
+template <> struct Held<float> { using type = f32x4; using any = f32x4_any; };
+template <> struct Held<bf16> {
+  using type = unsigned short __attribute__((ext_vector_type(4)));
+  using any = u16x4_any;
+};
+template <typename T>
+using held = typename Held<T>::type;
+
+__device__ __forceinline__ float widen(float v) { return v; }
+__device__ __forceinline__ float widen(unsigned short v) {
+  return __builtin_bit_cast(float, static_cast<unsigned>(v) << 16);
+}
+template <bool STREAM, typename T>
+__device__ __forceinline__ held<T> hold4(const T* p) {
+  const auto* q = reinterpret_cast<const typename Held<T>::any*>(p);
+  return STREAM ? __builtin_nontemporal_load(q) : *q;
+}
+// Values c .. c + 3 of a row of D, c a multiple of four that may lie past its end.  Where the row ends
+// first, its last four are loaded; widen_row moves them into place and gives zero for what is not there.
+// (Rows of fewer than four values are read one by one.)
+template <bool STREAM, typename T>
+__device__ __forceinline__ held<T> hold_row(const T* row, int c, int D) {
+  if (D >= 4) return hold4<STREAM>(row + (c <= D - 4 ? c : D - 4));
+  using U = std::conditional_t<sizeof(T) == 4, float, unsigned short>;
+  held<T> v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = c + i < D ? reinterpret_cast<const U*>(row)[c + i] : U(0);
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void widen_row(held<T> t, int c, int D, float (&v)[4]) {
+  const int by = D < 4 || c <= D - 4 ? 0 : c - (D - 4);
+  if constexpr (sizeof(T) == 2) {
+    const uint64_t w = by < 4 ? __builtin_bit_cast(uint64_t, t) >> (16 * by) : 0;
+    t = __builtin_bit_cast(held<T>, w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = widen(t[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = t[i];
+    if (D % 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = (by & 2) ? (i < 2 ? v[i + 2] : 0.0f) : v[i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = (by & 1) ? (i < 3 ? v[i + 1] : 0.0f) : v[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = by < 4 ? v[i] : 0.0f;
+  }
+}
+
+// Loads and stores of the last values of a row: `left` >= 1 of them exist, the others read as `fill`.
 template <bool STREAM = false, typename T>
 __device__ __forceinline__ void load4_upto(const T* p, int left, float fill, float (&v)[4]) {
   if (left >= 4) {

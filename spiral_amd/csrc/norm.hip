@@ -76,19 +76,30 @@ __device__ __forceinline__ float row_sum(float v, float* scratch, int& turn) {
 // width below which the kernel is not used, so the vectors below it exist without a question; the
 // lanes of the others may lie past the row's end, entirely or in part.
 template <int G, int R, int LO, bool STREAM, typename T>
-__device__ __forceinline__ void load_row(const T* src, int lane, int D, float fill, float (&v)[R][4]) {
+__device__ __forceinline__ void hold_all(const T* src, int lane, int D, held<T> (&t)[R]) {
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int c = (r * G + lane) * 4;
-    if ((r + 1) * G * 4 <= LO) {
-      load4<STREAM>(src + c, v[r]);
-    } else if (c < D) {
-      load4_upto<STREAM>(src + c, D - c, fill, v[r]);
-    } else {
+    t[r] = (r + 1) * G * 4 <= LO ? hold4<STREAM>(src + c) : hold_row<STREAM>(src, c, D);
+  }
+}
+template <int G, int R, int LO, typename T>
+__device__ __forceinline__ void widen_all(const held<T> (&t)[R], int lane, int D, float (&v)[R][4]) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[r][i] = fill;
+  for (int r = 0; r < R; ++r) {
+    if ((r + 1) * G * 4 <= LO) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[r][i] = widen(t[r][i]);
+    } else {
+      widen_row<T>(t[r], (r * G + lane) * 4, D, v[r]);
     }
   }
+}
+template <int G, int R, int LO, bool STREAM, typename T>
+__device__ __forceinline__ void load_row(const T* src, int lane, int D, float (&v)[R][4]) {
+  held<T> t[R];
+  hold_all<G, R, LO, STREAM>(src, lane, D, t);
+  widen_all<G, R, LO, T>(t, lane, D, v);
 }
 template <int G, int R, int LO, bool STREAM, typename T>
 __device__ __forceinline__ void store_row(T* dst, int lane, int D, const float (&v)[R][4]) {
@@ -116,7 +127,7 @@ __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_fwd_kernel(Fwd
   const float inv_d = 1.0f / static_cast<float>(p.D);
   float w[R][4], b[R][4];
   if (p.w) {
-    load_row<G, R, LO, false>(p.w, lane, p.D, 0.0f, w);
+    load_row<G, R, LO, false>(p.w, lane, p.D, w);
   } else {
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -124,7 +135,7 @@ __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_fwd_kernel(Fwd
       for (int i = 0; i < 4; ++i) w[r][i] = 1.0f;
   }
   if (p.b) {
-    load_row<G, R, LO, false>(p.b, lane, p.D, 0.0f, b);
+    load_row<G, R, LO, false>(p.b, lane, p.D, b);
   } else {
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -134,12 +145,15 @@ __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_fwd_kernel(Fwd
   for (int64_t first = static_cast<int64_t>(blockIdx.x) * (GROUPS * RU); first < p.M;
        first += static_cast<int64_t>(gridDim.x) * (GROUPS * RU)) {
     const int64_t row0 = first + grp;
+    held<T> raw[RU][R];
     float v[RU][R][4];
 #pragma unroll
     for (int u = 0; u < RU; ++u) {
       const int64_t row = row0 + u * GROUPS;  // past the end: the last row again, not stored
-      load_row<G, R, LO, true>(x + (row < p.M ? row : p.M - 1) * p.ldx, lane, p.D, 0.0f, v[u]);
+      hold_all<G, R, LO, true>(x + (row < p.M ? row : p.M - 1) * p.ldx, lane, p.D, raw[u]);
     }
+#pragma unroll
+    for (int u = 0; u < RU; ++u) widen_all<G, R, LO, T>(raw[u], lane, p.D, v[u]);
 #pragma unroll
     for (int u = 0; u < RU; ++u) {
       const int64_t row = row0 + u * GROUPS;
@@ -188,7 +202,7 @@ __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_bwd_kernel(Bwd
 
   float w[R][4], dw[R][4], db[R][4];
   if (p.w) {
-    load_row<G, R, LO, false>(p.w, lane, p.D, 0.0f, w);
+    load_row<G, R, LO, false>(p.w, lane, p.D, w);
   } else {
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -208,14 +222,18 @@ __global__ __launch_bounds__(G > kThreads ? G : kThreads) void ln_bwd_kernel(Bwd
     const int64_t at = there ? row : end - 1;
     const float2 st = p.stats[at];
     float xh[R][4], gv[R][4];
-    load_row<G, R, LO, true>(x + at * p.ldx, lane, p.D, st.x, xh);
-    load_row<G, R, LO, true>(g + at * p.ldg, lane, p.D, 0.0f, gv);
+    held<T> raw_x[R], raw_g[R];
+    hold_all<G, R, LO, true>(x + at * p.ldx, lane, p.D, raw_x);
+    hold_all<G, R, LO, true>(g + at * p.ldg, lane, p.D, raw_g);
+    widen_all<G, R, LO, T>(raw_x, lane, p.D, xh);
+    widen_all<G, R, LO, T>(raw_g, lane, p.D, gv);
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float h = (xh[r][i] - st.x) * st.y;
+        float h = (xh[r][i] - st.x) * st.y;
+        if ((r + 1) * G * 4 > LO && (r * G + lane) * 4 + i >= p.D) h = 0.0f;
         xh[r][i] = h;
         const float gi = there ? gv[r][i] : 0.0f;
         dw[r][i] = there ? __builtin_fmaf(gi, h, dw[r][i]) : dw[r][i];

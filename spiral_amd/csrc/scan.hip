@@ -26,8 +26,6 @@
 // is stored.  Steps where a node is not active pass the state (and its gradient) on unchanged;
 // what stands in the gates there is loaded but never used.
 
-#include <type_traits>
-
 #include "lanes.h"
 
 namespace {
@@ -114,17 +112,7 @@ struct Place {
   }
 };
 
-// Four values as they are stored.  The loads of several steps are issued without a branch or a conversion
-// between them, and widened when they are used: with either in between, each load is waited for before
-// the next is sent.  TINY: rows of fewer than four units.
-using f32x4_held = float __attribute__((ext_vector_type(4)));
-using u16x4_held = unsigned short __attribute__((ext_vector_type(4)));
-template <typename T> struct Held;
-template <> struct Held<float> { using type = f32x4_held; using any = f32x4_any; };
-template <> struct Held<bf16> { using type = u16x4_held; using any = u16x4_any; };
-template <typename T>
-using held = typename Held<T>::type;
-
+// TINY: rows of fewer than four units.
 template <bool STREAM, bool TINY, typename T>
 __device__ __forceinline__ held<T> take(const T* p, int left) {
   held<T> v;
@@ -133,14 +121,9 @@ __device__ __forceinline__ held<T> take(const T* p, int left) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = q[k < left ? k : left - 1];
   } else {
-    const auto* q = reinterpret_cast<const typename Held<T>::any*>(p);
-    v = STREAM ? __builtin_nontemporal_load(q) : *q;
+    v = hold4<STREAM>(p);
   }
   return v;
-}
-__device__ __forceinline__ float widen(float v) { return v; }
-__device__ __forceinline__ float widen(unsigned short v) {
-  return __builtin_bit_cast(float, static_cast<unsigned>(v) << 16);
 }
 template <bool TINY, typename T>
 __device__ __forceinline__ void put(T* p, int left, const float (&v)[4]) {
