@@ -67,18 +67,21 @@ __device__ __forceinline__ unsigned pack4(const float (&v)[4], float inv) {
   return inv == 0.0f ? 0u : lo | hi;
 }
 
-// q [M, width] (width >= K, zero past K) and the rows' scales.  A wave per row, which it keeps in
-// registers: R pieces of 64 lanes times 16 bytes (four values of float32, eight of bfloat16).  R = 0:
-// rows of any length, read twice.
-template <typename T, int R>
+// q [M, width] (width >= K, zero past K) and the rows' scales.  W waves per row, which keep it in
+// registers: R pieces of a lane each 16 bytes (four values of float32, eight of bfloat16).  R = 0: rows
+// of any length, read twice.
+template <typename T, int R, int W>
 __global__ __launch_bounds__(kThreads) void quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t M, int K,
                                                             int8_t* __restrict__ q, int64_t ldq, int width,
                                                             float* __restrict__ scale) {
   constexpr int V = 16 / sizeof(T) / 4;  // fours of a lane
-  constexpr int PIECE = 256 * V;
-  const int lane = threadIdx.x & 63;
-  for (int64_t row = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 6; row < M;
-       row += (static_cast<int64_t>(gridDim.x) * kThreads) >> 6) {
+  constexpr int ROWS = kThreads / (64 * W), PIECE = 256 * V * W;
+  static_assert(W == 1 || ROWS == 1, "the workgroup meets once a row");
+  __shared__ unsigned tops[W > 1 ? 2 : 1][W];
+  int turn = 0;
+  const int lane = threadIdx.x % (64 * W);
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + threadIdx.x / (64 * W); row < M;
+       row += static_cast<int64_t>(gridDim.x) * ROWS) {
     const T* const src = x + row * ldx;
     int8_t* const dst = q + row * ldq;
     unsigned top = 0;
@@ -94,6 +97,17 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const T* __restrict_
       }
     };
     float inv, s;
+    const auto agree = [&]() {
+      top = group_top<64>(top);
+      if constexpr (W > 1) {
+        if ((threadIdx.x & 63) == 0) tops[turn][threadIdx.x >> 6] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < W; ++i) top = tops[turn][i] > top ? tops[turn][i] : top;
+        turn ^= 1;
+      }
+      row_scale(top, inv, s);
+    };
     const auto put = [&](int c, const float (&v)[V][4]) {
       unsigned w[V];
 #pragma unroll
@@ -113,7 +127,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const T* __restrict_
       for (int r = 0; r < R; ++r) fetch(r * PIECE + lane * 4 * V, raw[r]);
 #pragma unroll
       for (int r = 0; r < R; ++r) look(r * PIECE + lane * 4 * V, raw[r], v[r]);
-      row_scale(group_top<64>(top), inv, s);
+      agree();
 #pragma unroll
       for (int r = 0; r < R; ++r) put(r * PIECE + lane * 4 * V, v[r]);
     } else {
@@ -124,7 +138,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const T* __restrict_
         fetch(c, raw);
         look(c, raw, v);
       }
-      row_scale(group_top<64>(top), inv, s);
+      agree();
 #pragma unroll 4
       for (int c = lane * 4 * V; c < width; c += PIECE) {
         fetch(c, raw);
@@ -840,8 +854,10 @@ int launch_few(const FewArgs& a, hipStream_t st) {
   if (a.M <= 32) return go(std::integral_constant<int, 2>{});
   return go(std::integral_constant<int, 4>{});
 }
-// Whole numbers that every workgroup of few_i8_kernel makes for itself.
-constexpr int64_t kFewMade = 16384;
+// Whole numbers that every workgroup of few_i8_kernel makes for itself (by 4096 columns, bfloat16): 16 x 2048
+// takes 13.2 us made there and 15.8 with a launch for them, 8 x 4096 14.0 and 15.8, but 16 x 4096 21.1
+// and 15.9, 32 x 1024 24.1 and 15.2.
+constexpr int64_t kFewMade = 32768;
 bool few_made(int64_t M, int64_t K) { return M <= 16 && M * K <= kFewMade; }
 
 int check_rows(const char* what, int dtype, int64_t M, int64_t K) {
@@ -856,17 +872,25 @@ int check_rows(const char* what, int dtype, int64_t M, int64_t K) {
 template <typename T>
 void launch_quantize(const void* x, int64_t ldx, int64_t M, int64_t K, int8_t* q, int64_t ldq, int64_t width,
                      float* scale, hipStream_t st) {
-  const auto go = [&](auto r) {
-    quantize_kernel<T, decltype(r)::value><<<static_cast<unsigned>((M + 3) / 4 < kMaxGroups ? (M + 3) / 4 : kMaxGroups), kThreads, 0, st>>>(
-        static_cast<const T*>(x), ldx, M, static_cast<int>(K), q, ldq, static_cast<int>(width), scale);
+  const auto go = [&](auto r, auto w) {
+    constexpr int W = decltype(w)::value, ROWS = kThreads / (64 * W);
+    const int64_t groups = (M + ROWS - 1) / ROWS;
+    quantize_kernel<T, decltype(r)::value, W>
+        <<<static_cast<unsigned>(groups < kMaxGroups ? groups : kMaxGroups), kThreads, 0, st>>>(
+            static_cast<const T*>(x), ldx, M, static_cast<int>(K), q, ldq, static_cast<int>(width), scale);
   };
-  const int64_t pieces = (width * static_cast<int64_t>(sizeof(T)) + 1023) / 1024;
-  if (pieces <= 1) go(std::integral_constant<int, 1>{});
-  else if (pieces <= 2) go(std::integral_constant<int, 2>{});
-  else if (pieces <= 4) go(std::integral_constant<int, 4>{});
-  else if (pieces <= 8) go(std::integral_constant<int, 8>{});
-  else if (sizeof(T) == 4 && pieces <= 16) go(std::integral_constant<int, sizeof(T) == 4 ? 16 : 0>{});
-  else go(std::integral_constant<int, 0>{});
+  using One = std::integral_constant<int, 1>;
+  using Four = std::integral_constant<int, 4>;
+  // Rows of up to four pieces go to one wave each, longer ones to four (the projection of 64 x 8192 to 2048
+  // columns in bfloat16 takes 25.7 us so and 33.5 with one, 8200 x 4096 to 512 in float32 64 and 68).
+  const int64_t pieces = (width * static_cast<int64_t>(sizeof(T)) + 1023) / 1024;  // of a wave
+  if (pieces <= 1) go(std::integral_constant<int, 1>{}, One{});
+  else if (pieces <= 2) go(std::integral_constant<int, 2>{}, One{});
+  else if (pieces <= 4) go(std::integral_constant<int, 4>{}, One{});
+  else if (pieces <= 8) go(std::integral_constant<int, 2>{}, Four{});
+  else if (pieces <= 16) go(std::integral_constant<int, 4>{}, Four{});
+  else if (pieces <= 32) go(std::integral_constant<int, 8>{}, Four{});
+  else go(std::integral_constant<int, 0>{}, Four{});
 }
 void launch_quantize(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, int8_t* q, int64_t ldq,
                      int64_t width, float* scale, hipStream_t st) {
