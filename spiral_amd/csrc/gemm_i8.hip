@@ -69,7 +69,7 @@ __device__ __forceinline__ unsigned pack4(const float (&v)[4], float inv) {
 
 // q [M, width] (width >= K, zero past K) and the rows' scales.  W waves per row, which keep it in
 // registers: R pieces of a lane each 16 bytes (four values of float32, eight of bfloat16).  R = 0: rows
-// of any length, read twice.
+// of any length, read twice.  Bound by memory: 8200 x 2048 in bfloat16 (50 MB) takes 13.2 us, 3.8 TB/s.
 template <typename T, int R, int W>
 __global__ __launch_bounds__(kThreads) void quantize_kernel(const T* __restrict__ x, int64_t ldx, int64_t M, int K,
                                                             int8_t* __restrict__ q, int64_t ldq, int width,
@@ -299,7 +299,8 @@ __device__ __forceinline__ void finish16(const i32x16& acc, const float (&sm)[16
 // Rows go from global memory into LDS directly, 16 bytes a lane, ST - 1 stages ahead of the products;
 // a stage is complete when the wave's own loads of it have landed (a counted wait) and a barrier
 // has told so for all waves, and that barrier also frees the buffer the next loads go to: one
-// barrier a stage.  An LDS row is 64 bytes, so a 16-lane group that reads 16 bytes of 16 rows meets
+// barrier a stage.  Bound by the matrix instructions and the LDS reads that feed them: 8192 x 4096 -> 4096 in
+// 140 us, 1964 x 10^12 operations a second.  An LDS row is 64 bytes, so a 16-lane group that reads 16 bytes of 16 rows meets
 // each bank four times unless the four pieces of a row are turned by the row's number / 4: the loads
 // fetch them in that order.  Rows past the end repeat the last one and are not stored.
 template <typename OUT, int BM, int BN, int WM, int WN, int ST>
@@ -468,10 +469,11 @@ __global__ __launch_bounds__(WM * WN * 64) void tile_i8_kernel(GemmArgs p) {
 //
 // The kernel is bound by memory: x is read once, results are written once, 128 contiguous bytes of a
 // row at a time, both marked as streams (10^5 x 512 -> 1024: 179 us without, 152 with), and the weight
-// comes from L2 once per 256 rows: 10^6 x 128 -> 256 in float32 takes 290 us, 5.3 TB/s.  Workgroups are short (256 rows): handed out in order, they keep what is in flight
-// close together in memory, which is worth a tenth against a resident grid that strides over the
-// rows.  They begin at different columns: 96 us instead of 124 at 10^5 x 128 -> 1024.  LDS rows are padded by 16 bytes: 16 lanes that read 16 bytes of 16 neighbouring rows then meet each
-// bank once.
+// comes from L2 once per 256 rows: 10^6 x 128 -> 256 in float32 takes 290 us, 5.3 TB/s.  Workgroups are
+// short (256 rows): handed out in order, they keep what is in flight close together in memory, which is worth
+// a tenth against a resident grid that strides over the rows.  They begin at different columns: 96 us instead
+// of 124 at 10^5 x 128 -> 1024.  LDS rows are padded by 16 bytes: 16 lanes that read 16 bytes of 16
+// neighbouring rows then meet each bank once.
 template <int KP>
 struct RowsShape {
   static constexpr int NW = 8, SK = KP + 16;
@@ -647,7 +649,8 @@ __global__ __launch_bounds__(RowsShape<KP>::NW * 64, 2) void rows_i8_kernel(Rows
 // waves take turns at the 64-byte pieces of K, reading them from memory straight into the operand
 // layout (16 rows, 16 neighbouring k a lane), and add their sums up in LDS at the end.  The rows are
 // brought to whole numbers in LDS by every workgroup for itself (T float or bfloat16: a launch less,
-// and a small x comes from L2), or come from a matrix made before (T int8_t: larger x).
+// and a small x comes from L2), or come from a matrix made before (T int8_t: larger x).  Four loads a
+// wave are ahead of the products (eight: 8 x 8192 -> 8192 takes 30 us, not 21).
 struct FewArgs {
   const void* x;         // [M, K] values, or whole numbers zero from K to the next multiple of 64
   int64_t ldx;
@@ -666,13 +669,23 @@ struct FewArgs {
 constexpr int kFewWaves = 8;
 constexpr int kFewRows = 64;
 
-template <typename T, typename OUT, int MT>
+// Pieces of a workgroup's width that M rows of K values take, and how many of them it holds: the rows are
+// loaded at once and stay in registers.  By 4096 columns in bfloat16, 16 rows of 2048 take 11.1 us a call so
+// and 14.4 with a launch of their own for the whole numbers, 8 of 4096 13.2 and 15.8; but twice the pieces in
+// two turns, 16 of 4096, took 21.1 where the launch takes 15.9.
+constexpr int kFewPiece = kFewWaves * 256;
+constexpr int kFewPieces = 16;
+
+// P: pieces held (T float or bfloat16); MT: rows, in sixteens.
+template <typename T, typename OUT, int MT, int P>
 __global__ __launch_bounds__(kFewWaves * 64) void few_i8_kernel(FewArgs p) {
   constexpr bool MAKE = sizeof(T) > 1;
   constexpr int NW = kFewWaves, U = 4;
+  static_assert(MAKE ? P > 0 && P <= kFewPieces && MT == 1 : P == 0, "pieces");
   __shared__ i32x4 sums[NW][MT][64];
   __shared__ float row_scale_of[16 * MT];
-  __shared__ unsigned tops[MAKE ? 16 * MT : 1][NW];
+  __shared__ unsigned tops[MAKE ? P : 1][NW];
+  __shared__ float inv_of[16];
   extern __shared__ i32x4 smem[];
   char* const q = reinterpret_cast<char*>(smem);  // MAKE: rows of KP + 16 bytes
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -692,48 +705,47 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_i8_kernel(FewArgs p) {
 
   const T* const x = static_cast<const T*>(p.x);
   if constexpr (MAKE) {
-    for (int r0 = 0; r0 < p.M; r0 += 4) {
-      unsigned top[4] = {0, 0, 0, 0};
-      for (int c = tid * 4; c < p.K; c += NW * 256) {
-        held<T> raw[4];
+    const int per = (p.K + kFewPiece - 1) / kFewPiece;  // pieces of a row; those of all rows are on the way together
+    held<T> raw[P];
+    {
+      int r = 0, i = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) raw[j] = hold_row<false>(x + (r0 + j < p.M ? r0 + j : r0) * p.ldx, c, p.K);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float v[4];
-          widen_row<T>(raw[j], c, p.K, v);
-          top[j] = top_of(top[j], v);
+      for (int k = 0; k < P; ++k) {
+        raw[k] = hold_row<false>(x + r * p.ldx, i * kFewPiece + tid * 4, p.K);
+        if (++i == per) {
+          i = 0;
+          r = r + 1 < p.M ? r + 1 : r;  // past the last row: it again, not used
         }
       }
+      i = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        top[j] = group_top<64>(top[j]);
-        if (lane == 0 && r0 + j < p.M) tops[r0 + j][wave] = top[j];
+      for (int k = 0; k < P; ++k) {
+        float v[4];
+        widen_row<T>(raw[k], i * kFewPiece + tid * 4, p.K, v);
+        const unsigned top = group_top<64>(top_of(0, v));
+        if (lane == 0) tops[k][wave] = top;
+        i = i + 1 < per ? i + 1 : 0;
       }
     }
     __syncthreads();
-    for (int r0 = 0; r0 < p.M; r0 += 4) {
-      float inv[4];
+    if (tid < p.M) {
+      unsigned top = 0;
+      for (int k = tid * per; k < tid * per + per; ++k)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int r = r0 + j < p.M ? r0 + j : r0;
-        unsigned top = tops[r][0];
-        float s;
+        for (int i = 0; i < NW; ++i) top = tops[k][i] > top ? tops[k][i] : top;
+      row_scale(top, inv_of[tid], row_scale_of[tid]);
+    }
+    __syncthreads();
+    int r = 0, i = 0;
 #pragma unroll
-        for (int i = 1; i < NW; ++i) top = tops[r][i] > top ? tops[r][i] : top;
-        row_scale(top, inv[j], s);
-        if (tid == 0) row_scale_of[r] = s;
-      }
-      for (int c = tid * 4; c < KP; c += NW * 256) {
-        held<T> raw[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) raw[j] = hold_row<false>(x + (r0 + j < p.M ? r0 + j : r0) * p.ldx, c, p.K);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float v[4];
-          widen_row<T>(raw[j], c, p.K, v);
-          if (r0 + j < p.M) *reinterpret_cast<unsigned*>(q + (r0 + j) * SK + c) = pack4(v, inv[j]);
-        }
+    for (int k = 0; k < P; ++k) {
+      const int c = i * kFewPiece + tid * 4;
+      float v[4];
+      widen_row<T>(raw[k], c, p.K, v);
+      if (r < p.M && c < KP) *reinterpret_cast<unsigned*>(q + r * SK + c) = pack4(v, inv_of[r]);
+      if (++i == per) {
+        i = 0;
+        ++r;
       }
     }
     __syncthreads();
@@ -824,7 +836,9 @@ int launch_tile(const GemmArgs& a, hipStream_t st) {
   return SPMI_OK;
 }
 // A CU's share of the work with tiles of an area: how many of them the busiest CU gets.  Tiles of
-// 256 x 256 move the least through LDS and L2, smaller ones leave fewer CUs idle at the end.
+// 256 x 256 move the least through LDS and L2, smaller ones leave fewer CUs idle at the end: the product
+// of 8200 x 2048 -> 4096 takes 107 us in tiles of 256 x 256 (a third round for 16 of 528 tiles), 101 of
+// 128 x 128 and 94 of 192 x 256.  The weights are what the smaller tiles cost more per output.
 template <typename OUT>
 int launch_tiles(const GemmArgs& a, hipStream_t st) {
   const auto share = [&](int64_t bm, int64_t bn, double weight) {
@@ -839,26 +853,34 @@ int launch_tiles(const GemmArgs& a, hipStream_t st) {
   return launch_tile<OUT, 256, 256, 2, 4, 4>(a, st);
 }
 
+int64_t few_pieces(int64_t M, int64_t K) { return M * ((K + kFewPiece - 1) / kFewPiece); }
+
 template <typename T, typename OUT>
 int launch_few(const FewArgs& a, hipStream_t st) {
   const unsigned grid = static_cast<unsigned>((a.N + 15) / 16);
-  const auto go = [&](auto mt) {
+  const auto go = [&](auto mt, auto pieces) {
     constexpr int MT = decltype(mt)::value;
     const size_t lds = sizeof(T) > 1 ? static_cast<size_t>(a.M) * (((a.K + 63) & ~63) + 16) : 0;
-    const auto kernel = few_i8_kernel<T, OUT, MT>;
+    const auto kernel = few_i8_kernel<T, OUT, MT, decltype(pieces)::value>;
     SPMI_RAISE_LDS_LIMIT(kernel, lds);
     kernel<<<grid, kFewWaves * 64, lds, st>>>(a);
     return SPMI_OK;
   };
-  if (a.M <= 16) return go(std::integral_constant<int, 1>{});
-  if (a.M <= 32) return go(std::integral_constant<int, 2>{});
-  return go(std::integral_constant<int, 4>{});
+  using One = std::integral_constant<int, 1>;
+  if constexpr (sizeof(T) > 1) {
+    const int64_t pieces = few_pieces(a.M, a.K);
+    if (pieces <= 1) return go(One{}, One{});
+    if (pieces <= 4) return go(One{}, std::integral_constant<int, 4>{});
+    return go(One{}, std::integral_constant<int, kFewPieces>{});
+  } else {
+    using None = std::integral_constant<int, 0>;
+    if (a.M <= 16) return go(One{}, None{});
+    if (a.M <= 32) return go(std::integral_constant<int, 2>{}, None{});
+    return go(std::integral_constant<int, 4>{}, None{});
+  }
 }
-// Whole numbers that every workgroup of few_i8_kernel makes for itself (by 4096 columns, bfloat16): 16 x 2048
-// takes 13.2 us made there and 15.8 with a launch for them, 8 x 4096 14.0 and 15.8, but 16 x 4096 21.1
-// and 15.9, 32 x 1024 24.1 and 15.2.
-constexpr int64_t kFewMade = 32768;
-bool few_made(int64_t M, int64_t K) { return M <= 16 && M * K <= kFewMade; }
+// Rows that every workgroup of few_i8_kernel brings to whole numbers for itself.
+bool few_made(int64_t M, int64_t K) { return few_pieces(M, K) <= kFewPieces; }
 
 int check_rows(const char* what, int dtype, int64_t M, int64_t K) {
   SPMI_REQUIRE(dtype == SPMI_DTYPE_F32 || dtype == SPMI_DTYPE_BF16, SPMI_ERR_INVALID_ARG, "%s: dtype %d", what, dtype);

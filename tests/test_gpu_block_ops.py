@@ -552,6 +552,17 @@ def test_linear_int8_sizes(dev, m, k, n, dtype):
     check_int8(x, wq, ws, None, "leaky_relu", 0.2, BF16 if dtype == F32 else F32)
 
 
+# rows on both sides of what a workgroup holds of them (16 pieces of 2048 values), of the pieces a wave
+# or four waves hold, and of rows that are read twice
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("m,k,n", [(8, 4096, 40), (8, 4097, 40), (5, 4098, 17), (1, 32768, 20), (1, 32769, 5), (3, 9000, 33),
+                                   (2, 16384, 16), (2, 16390, 16), (16, 1, 3), (16, 3, 20), (15, 2047, 50), (65, 8193, 20),
+                                   (70, 16385, 9), (20, 1025, 30), (18, 2049, 31), (100, 5000, 70)])
+def test_linear_int8_long_rows(dev, m, k, n, dtype):
+    wq, ws = weight8(n, k)
+    check_int8(rand(m, k, dtype=dtype, seed=m + k + n), wq, ws, rand(n, seed=1))
+
+
 def test_linear_int8_activations_bias_types_and_shapes(dev):
     wq, ws = weight8(40, 72)
     x = rand(4, 9, 72)
