@@ -670,6 +670,9 @@ int spmi_bn_bwd_apply(const float* dy, const float* z, int64_t M, int64_t W, int
                       const float* stats, const float* sums, float* dz, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Operators of a gated-linear-recurrence decoder block (this group and the next two).  What a call
+ * writes may not overlap what it reads, but for the memory of spmi_gated_step.
+ *
  * Layer norm of rows: y = (x - mean) r w + b with r = (variance + eps)^-1/2, the variance taken
  * over the row's D values (1 <= D <= spmi_layer_norm_max_width()).  x and y are float32 or
  * bfloat16 (`dtype`) with row strides in values (0 repeats one row; any alignment), w and b

@@ -14,6 +14,10 @@
 // row its group visits, so it adds them up in registers; the groups of a workgroup meet in LDS,
 // the workgroups in a second launch that adds their partial rows in a fixed order.  No atomics:
 // the same call gives the same bits.
+//
+// 10^6 x 128 in float32: 1.02 GB forward in 171-178 us (5.8-6.0 TB/s), 1.54 GB backward in 260-265 us and
+// 11 us for the sums; a copy of that size in the same kind of grid reaches 6.7 TB/s.  12289 x 1031 in
+// bfloat16 (rows that start at odd addresses): 51 MB in 17 us, 76 MB in 22.5 us and 4.
 
 #include "lanes.h"
 
