@@ -269,6 +269,19 @@ def test_scan_many_lanes(dev, dtype):
     check_scan(rand(t, n, 2 * h, dtype=dtype), rand(n, h, seed=1), make_active(t, n))
 
 
+# rows of fewer than four units, and of a few more, in each layout: walked (few steps; many lanes), strands of
+# enough workgroups to leave the steps whole, and split steps
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("t,n,h", [(3, 50, 1), (5, 7, 2), (19, 70000, 3), (21, 66000, 2), (23, 33000, 5), (40, 17000, 3),
+                                   (37, 4200, 14), (700, 3, 2), (901, 2, 3), (1200, 1, 1), (333, 5, 7)])
+def test_scan_short_rows_in_every_layout(dev, t, n, h, dtype):
+    gates = rand(t, n, 2 * h, dtype=dtype, seed=t + n + h)
+    on = make_active(t, n)
+    check_scan(gates, rand(n, h, seed=1), on)
+    check_scan(gates.masked_fill(~on[..., None], float("nan")), None, on, with_g=False)
+    check_scan(gates.transpose(0, 1).contiguous(), rand(n, h, seed=2), on.t(), batch_first=True)
+
+
 @pytest.mark.parametrize("t,n,h", [(33, 5, 12), (300, 2, 128), (9, 70, 30)])
 def test_scan_batch_first_and_strides(dev, t, n, h):
     on = make_active(t, n)
