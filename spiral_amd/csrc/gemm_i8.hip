@@ -879,8 +879,14 @@ int launch_few(const FewArgs& a, hipStream_t st) {
     return go(std::integral_constant<int, 4>{}, None{});
   }
 }
-// Rows that every workgroup of few_i8_kernel brings to whole numbers for itself.
-bool few_made(int64_t M, int64_t K) { return few_pieces(M, K) <= kFewPieces; }
+// Rows that every workgroup of few_i8_kernel brings to whole numbers for itself: as many as it holds, and not so
+// many columns that the repetition costs more than a launch (16 x 1024 in bfloat16 to 8192 columns 12.0 us
+// against 14.7, to 16384 20.9 against 14.8; 4 x 1024 to 50000 26.4 against 18.5; one row to 50000 17.4
+// against 17.7).
+bool few_made(int64_t M, int64_t K, int64_t N) {
+  const int64_t pieces = few_pieces(M, K);
+  return pieces == 1 || (pieces <= kFewPieces && pieces * N <= 131072);
+}
 
 int check_rows(const char* what, int dtype, int64_t M, int64_t K) {
   SPMI_REQUIRE(dtype == SPMI_DTYPE_F32 || dtype == SPMI_DTYPE_BF16, SPMI_ERR_INVALID_ARG, "%s: dtype %d", what, dtype);
@@ -937,7 +943,7 @@ int spmi_quantize_rows_i8(const void* x, int dtype, int64_t ldx, int64_t M, int6
 
 size_t spmi_linear_i8_workspace_bytes(int64_t M, int64_t K, int64_t N) {
   if (M <= 0 || K <= 0 || N <= 0) return 0;
-  if (few_made(M, K) || rows_take(M, K)) return 0;
+  if (few_made(M, K, N) || rows_take(M, K)) return 0;
   // whole numbers of x, their scales, the weight in rows of whole stages (not needed if it has them)
   return align_up(static_cast<size_t>(M) * padded(K), 256) + align_up(static_cast<size_t>(M) * sizeof(float), 256) +
          (static_cast<size_t>(N) * padded(K));
@@ -959,7 +965,7 @@ int spmi_linear_i8(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, 
                "spmi_linear_i8: null pointer or row stride too small");
   hipStream_t st = as_stream(stream);
   const bool f32 = dtype == SPMI_DTYPE_F32, of32 = out_dtype == SPMI_DTYPE_F32;
-  if (few_made(M, K) || rows_take(M, K)) {  // one launch
+  if (few_made(M, K, N) || rows_take(M, K)) {  // one launch
     int rc;
     if (M <= kFewRows) {
       const FewArgs a{x, ldx, nullptr, static_cast<int>(M), weight, ldw, N, static_cast<int>(K), w_scale, bias, act, slope,

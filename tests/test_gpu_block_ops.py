@@ -576,6 +576,15 @@ def test_linear_int8_long_rows(dev, m, k, n, dtype):
     check_int8(rand(m, k, dtype=dtype, seed=m + k + n), wq, ws, rand(n, seed=1))
 
 
+# few rows by so many columns that they are brought to whole numbers in a launch of their own, and just below
+@pytest.mark.parametrize("m,k,n", [(16, 100, 8192), (16, 100, 8193), (3, 65, 43690), (3, 65, 43691), (1, 40, 140000),
+                                   (2, 40, 65537)])
+def test_linear_int8_few_rows_many_columns(dev, m, k, n):
+    wq, ws = weight8(n, k)
+    check_int8(rand(m, k, dtype=BF16, seed=m + k + n), wq, ws, rand(n, seed=1))
+    check_int8(rand(m, k, seed=m + k + n), wq, ws, None, "relu")
+
+
 def test_linear_int8_activations_bias_types_and_shapes(dev):
     wq, ws = weight8(40, 72)
     x = rand(4, 9, 72)
