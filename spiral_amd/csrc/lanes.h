@@ -108,10 +108,10 @@ __device__ __forceinline__ void widen_row(held<T> t, int c, int D, float (&v)[4]
 }
 
 // Loads and stores of the last values of a row: `left` >= 1 of them exist, the others read as `fill`.
-template <bool STREAM = false, typename T>
+template <typename T>
 __device__ __forceinline__ void load4_upto(const T* p, int left, float fill, float (&v)[4]) {
   if (left >= 4) {
-    load4<STREAM>(p, v);
+    load4(p, v);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = i < left ? static_cast<float>(p[i]) : fill;
