@@ -699,8 +699,12 @@ int spmi_layer_norm_bwd(const void* x, const void* g, int dtype, int64_t ldx, in
  *   active   nullable, one byte per step and node (strides in bytes): where it is 0 the state
  *            passes unchanged and the gates are not used (their gradient is 0)
  *   last     float32 [N, H]: the state after the last step (h0 if T = 0)
- *   bwd      g, g_last (nullable: zeros) = gradients of h and last; h as the forward wrote it (not
- *            read if T <= 1) -> dgates, dh0 (nullable, [N, H])
+ *   states   nullable, float32 [spmi_gated_scan_states(T, N, H), N, H]: the state after every few
+ *            steps, whole.  The backward pass of bfloat16 gates needs them: the gate's gradient
+ *            takes the difference h_{t-1} - c, of which a state rounded to bfloat16 can leave little
+ *   bwd      g, g_last (nullable: zeros) = gradients of h and last; float32: h as the forward wrote
+ *            it (not read if T <= 1), bfloat16: states -> dgates, dh0
+ *            (nullable, [N, H])
  *   ws       the matching _workspace_bytes (0 for most sizes), aligned to 16 bytes
  * spmi_gated_step is one step on rows of the node memory h_mem [nodes, H] (contiguous): row i
  * belongs to node ids[i] (NULL: i); h_out float32 [M, H] gets the new states, h_before (nullable)
@@ -713,10 +717,15 @@ size_t spmi_gated_scan_bwd_workspace_bytes(int64_t T, int64_t N, int64_t H);
 int spmi_gated_scan_fwd(const void* gates, int dtype, int64_t gates_t, int64_t gates_n, const float* h0, int64_t h0_n,
                         const uint8_t* active, int64_t active_t, int64_t active_n, int64_t T, int64_t N, int64_t H,
                         void* h, int64_t h_t, int64_t h_n, float* last, void* ws, size_t ws_bytes, void* stream);
+int64_t spmi_gated_scan_states(int64_t T, int64_t N, int64_t H);
+int spmi_gated_scan_fwd_saved(const void* gates, int dtype, int64_t gates_t, int64_t gates_n, const float* h0,
+                              int64_t h0_n, const uint8_t* active, int64_t active_t, int64_t active_n, int64_t T,
+                              int64_t N, int64_t H, void* h, int64_t h_t, int64_t h_n, float* last, float* states,
+                              void* ws, size_t ws_bytes, void* stream);
 int spmi_gated_scan_bwd(const void* gates, int dtype, int64_t gates_t, int64_t gates_n, const float* h0, int64_t h0_n,
                         const uint8_t* active, int64_t active_t, int64_t active_n, int64_t T, int64_t N, int64_t H,
-                        const void* h, int64_t h_t, int64_t h_n, const void* g, int64_t g_t, int64_t g_n,
-                        const float* g_last, int64_t gl_n, void* dgates, int64_t dg_t, int64_t dg_n, float* dh0,
+                        const void* h, int64_t h_t, int64_t h_n, const float* states, const void* g, int64_t g_t,
+                        int64_t g_n, const float* g_last, int64_t gl_n, void* dgates, int64_t dg_t, int64_t dg_n, float* dh0,
                         void* ws, size_t ws_bytes, void* stream);
 size_t spmi_gated_step_workspace_bytes(int64_t M, int64_t nodes);
 int spmi_gated_step(const void* gates, int dtype, int64_t ldg, float* h_mem, int64_t nodes, const int64_t* ids,

@@ -136,9 +136,12 @@ _SIGNATURES = {
     "spmi_gated_scan_bwd_workspace_bytes": (c_sz, [c_i64, c_i64, c_i64]),
     "spmi_gated_scan_fwd": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64,
                                     c_vp, c_i64, c_i64, c_vp, c_vp, c_sz, c_vp]),
+    "spmi_gated_scan_states": (c_i64, [c_i64, c_i64, c_i64]),
+    "spmi_gated_scan_fwd_saved": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_i64,
+                                          c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_sz, c_vp]),
     "spmi_gated_scan_bwd": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64,
-                                    c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_vp,
-                                    c_vp, c_sz, c_vp]),
+                                    c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64,
+                                    c_vp, c_vp, c_sz, c_vp]),
     "spmi_gated_step_workspace_bytes": (c_sz, [c_i64, c_i64]),
     "spmi_gated_step": (c_int, [c_vp, c_int, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_int, c_vp, c_sz,
                                 c_vp]),

@@ -204,16 +204,16 @@ def _scan_sizes(gates, h0, active, batch_first, h):
             (t, n, gates.shape[2] // 2), _step_strides(h, batch_first))
 
 
-def _scan_bwd(gates, h0, active, batch_first, code, at, h, g, g_last, dgates, dh0, sizes, ws_bytes):
+def _scan_bwd(gates, h0, active, batch_first, code, at, h, states, g, g_last, dgates, dh0, sizes, ws_bytes):
     of_gates, of_h0, of_active, tnh, of_h = sizes
     ws = _workspace(ws_bytes, gates.device)
     _launch("spmi_gated_scan_bwd", at, gates.data_ptr(), code, *of_gates, _ptr(h0), of_h0, _ptr(active), *of_active,
-            *tnh, h.data_ptr(), *of_h, _ptr(g), *_step_strides(g, batch_first), _ptr(g_last),
+            *tnh, _ptr(h), *of_h, _ptr(states), _ptr(g), *_step_strides(g, batch_first), _ptr(g_last),
             0 if g_last is None else g_last.stride(0), _ptr(dgates), *_step_strides(dgates, batch_first), _ptr(dh0),
             _ptr(ws), ws_bytes)
 
 
-def _scan_fwd(gates, h0, active, batch_first, code, at):
+def _scan_fwd(gates, h0, active, batch_first, code, at, keep):
     gates = _units_last(gates)
     if h0 is not None:
         h0 = _units_last(h0)
@@ -224,23 +224,27 @@ def _scan_fwd(gates, h0, active, batch_first, code, at):
     last = _empty(tnh[1:], dtype=_F32, device=dev)
     ws_bytes = nv.lib().spmi_gated_scan_fwd_workspace_bytes(*tnh)
     ws = _workspace(ws_bytes, dev)
-    _launch("spmi_gated_scan_fwd", at, gates.data_ptr(), code, *of_gates, _ptr(h0), of_h0, _ptr(active), *of_active,
-            *tnh, h.data_ptr(), *of_h, last.data_ptr(), _ptr(ws), ws_bytes)
-    return h, last, sizes
+    # float32 states are whole in h; of those stored in bfloat16 the backward pass gets some in float32 as well
+    states = None
+    if keep and gates.dtype != _F32:
+        states = _empty(nv.lib().spmi_gated_scan_states(*tnh), *tnh[1:], dtype=_F32, device=dev)
+    _launch("spmi_gated_scan_fwd_saved", at, gates.data_ptr(), code, *of_gates, _ptr(h0), of_h0, _ptr(active),
+            *of_active, *tnh, h.data_ptr(), *of_h, last.data_ptr(), _ptr(states), _ptr(ws), ws_bytes)
+    return h, last, states, sizes
 
 
 class _GatedScan(_Operator):
     @staticmethod
     def forward(ctx, gates, h0, active, batch_first, code, at):
-        h, last, sizes = _scan_fwd(gates, h0, active, batch_first, code, at)
-        ctx.save_for_backward(gates, h0, active, h)
+        h, last, states, sizes = _scan_fwd(gates, h0, active, batch_first, code, at, True)
+        ctx.save_for_backward(gates, h0, active, h if states is None else None, states)
         ctx.plain = (batch_first, code, at, sizes, nv.lib().spmi_gated_scan_bwd_workspace_bytes(*sizes[3]))
         ctx.set_materialize_grads(False)
         return h, last
 
     @staticmethod
     def gradients(ctx, g, g_last):
-        gates, h0, active, h = ctx.saved_tensors
+        gates, h0, active, h, states = ctx.saved_tensors
         batch_first, code, at, sizes, ws_bytes = ctx.plain
         need_gates, need_h0 = ctx.needs_input_grad[:2]
         if g is None and g_last is None:
@@ -250,7 +254,7 @@ class _GatedScan(_Operator):
             h0 = _units_last(h0)
         dgates = _empty(gates.shape, dtype=gates.dtype, device=gates.device) if need_gates else None
         dh0 = _empty(h0.shape, dtype=_F32, device=gates.device) if need_h0 else None
-        _scan_bwd(gates, h0, active, batch_first, code, at, h, None if g is None else _units_last(g),
+        _scan_bwd(gates, h0, active, batch_first, code, at, h, states, None if g is None else _units_last(g),
                   None if g_last is None else _units_last(g_last), dgates, dh0, sizes, ws_bytes)
         return dgates, dh0, None, None, None, None
 
@@ -285,7 +289,7 @@ def gated_scan(gates: torch.Tensor, h0: Optional[torch.Tensor] = None, active: O
     at = _device_of(gates, h0, active)
     if grad and _tracking():
         return _GatedScan.apply(gates, h0, active, batch_first, code, at)
-    return _scan_fwd(gates, h0, active, batch_first, code, at)[:2]
+    return _scan_fwd(gates, h0, active, batch_first, code, at, False)[:2]
 
 
 def _step_fwd(gates, h_mem, ids, mem_write, code, at, keep):
@@ -319,7 +323,7 @@ class _GatedStep(_Operator):
         dgates = _empty(gates.shape, dtype=gates.dtype, device=gates.device)
         m, h2 = gates.shape
         sizes = ((0, gates.stride(0)), h2 // 2, (0, 0), (1, m, h2 // 2), (0, 0))
-        _scan_bwd(gates, before, None, False, *ctx.plain, before, None, _units_last(g), dgates[None], None, sizes, 0)
+        _scan_bwd(gates, before, None, False, *ctx.plain, None, None, None, _units_last(g), dgates[None], None, sizes, 0)
         return dgates, None, None, None, None, None
 
 

@@ -8,8 +8,8 @@
 // Nothing here depends on h but h itself, so both directions are a chain of maps v -> p v + q that
 // can be joined pairwise: a stretch of steps is one such map (p = product of the a, q = what the
 // stretch makes of zero).  Both are bound by memory (forward: two values in, one out per unit and
-// step; backward: four in, two out), and the design is about having enough loads in flight while
-// every value is read once:
+// step; backward: three in, two out, and a state for every group of steps), and the design is about
+// having enough loads in flight while every value is read once:
 //  * many channels: a thread owns four neighbouring units of one node and walks the steps; the
 //    loads of several steps are issued together;
 //  * few channels (a long sequence of one or a few nodes): a workgroup is 8 strands of 32 lanes.
@@ -23,8 +23,14 @@
 //
 // a and 1 - a are computed from exp(-|z|), so neither loses digits where it is small; the state, its
 // gradient and the maps are float32 whatever the storage type, and a state is rounded only when it
-// is stored.  Steps where a node is not active pass the state (and its gradient) on unchanged;
-// what stands in the gates there is loaded but never used.
+// is stored for the caller.  dz takes the difference h_{t-1} - c, which cancels where a state follows its
+// candidates, so the backward pass reads no rounded state: it makes the states of a group of steps again,
+// by the forward pass's arithmetic, from the float32 state before the group.  That is the row of h itself
+// in float32; for bfloat16 the forward pass leaves it beside h, one state for 4 steps walked (half a value
+// of bfloat16 a step) and for 2 of a strand.
+//
+// Steps where a node is not active pass the state (and its gradient) on unchanged; what stands in the
+// gates there is never used.
 
 #include "lanes.h"
 
@@ -34,16 +40,19 @@ using namespace spmi;
 
 constexpr int kThreads = 256;
 // Steps a thread holds in registers.  Walking, the loads of the next steps are sent before the stores of
-// the present ones: 32 x 50000 x 128 takes 481 us forward and 1388 trained in float32, 244 and 690 in
-// bfloat16 (without: 494, 1431, 246, 704; with 2 steps forward 488, 1410).  As one of the strands, other
-// waves cover the wait better than registers do (four waves to a SIMD: 1185 x 2255 x 30 trained in
-// bfloat16 539 us, with six 765), and more steps pay less than they cost: 65536 x 1 x 128 42 us with 2
-// forward, 49 with 4; 1601 x 717 x 64 trained in float32 692 with 2 backward, 819 with 4.
+// the present ones: 32 x 50000 x 128 takes 481 us forward and 1279 trained in float32, 238 and 670 in
+// bfloat16 (with 2 steps backward 1319 and 767; forward in float32 without the loads ahead 494, with 2
+// steps 488).  As one of the strands, other waves cover the wait better than registers do (1185 x 2255 x 30
+// trained in bfloat16 takes 475 us with four waves to a SIMD; with six the registers spill, 1.4 times as
+// long), and more steps pay less than they cost: 65536 x 1 x 128 42 us with 2 forward, 49 with 4;
+// 1601 x 717 x 64 trained in float32 663 with 2 backward, 1.2 times as long with 4.
 constexpr int kFwdSteps = 2;
 constexpr int kFwdWalkSteps = 4;
 constexpr int kBwdSteps = 2;
-template <typename T>
-constexpr int kBwdWalkSteps = sizeof(T) == 4 ? 4 : 2;
+constexpr int kBwdWalkSteps = 4;
+// Backward they are also a group: the states inside one are made again from the one before it.
+template <bool WALK>
+constexpr int kGroup = WALK ? kBwdWalkSteps : kBwdSteps;
 constexpr int kLanes = 32;     // shape of a workgroup over few channels: lanes x strands
 constexpr int kStrands = kThreads / kLanes;
 // Threads (of four units) from which the steps are walked by one thread each: one wave per SIMD.
@@ -52,7 +61,7 @@ constexpr int64_t kManyLanes = 65536;
 constexpr int64_t kFewSteps = 16;
 // Workgroups from which the steps are not split: two per CU (852 x 221 x 448 in bfloat16, 774 workgroups, takes
 // 139 us unsplit and 188 in two, which read the gates twice).  Below, as many splits as make kTargetGroups
-// (1601 x 717 x 64, 359 workgroups, trained in bfloat16 406 us in five, 478 in two).
+// (1601 x 717 x 64, 359 workgroups, trained in bfloat16 404 us in five, a sixth longer in two).
 constexpr int64_t kEnoughGroups = 512;
 constexpr int64_t kTargetGroups = 2048;
 constexpr int64_t kMaxSplits = 512;
@@ -64,9 +73,12 @@ struct ScanArgs {
   int64_t h0_n;
   const uint8_t* active;  // nullable, [T, N]
   int64_t active_t, active_n;
-  void* h;             // [T, N, H]: written forward, read backward
+  void* h;             // forward: [T, N, H]
   int64_t h_t, h_n;
   float* last;         // forward: [N, H]
+  float* states;       // forward, nullable, [groups - 1, N, H]: the state before each group but the first
+  const float* before; // backward: the same, with strides before_g, before_n (null if there is one group)
+  int64_t before_g, before_n;
   const void* g;       // backward, nullable: gradient of h
   int64_t g_t, g_n;
   const float* g_last; // backward, nullable, [N, H]
@@ -151,7 +163,7 @@ __global__ __launch_bounds__(kThreads, S > 1 ? 4 : 1) void scan_fwd_kernel(ScanA
   // The loads of all steps are in flight together: steps past the end read the last one again, lanes past
   // the end the first node's; `on` says what counts.  Walking, a thread knows a tile ahead which steps are
   // active (`ahead`) and leaves out the rows of the others without a wait: 32 x 50000 x 128 with about a quarter
-  // of them inactive, trained in float32, 1183 us instead of 1384.  As a strand it reads them (852 x 221 x 448
+  // of them inactive, trained in float32, 1105 us instead of 1279.  As a strand it reads them (852 x 221 x 448
   // in bfloat16, ragged: 144 us, with the questions between the loads 171).
   held<T> raw_z[L], raw_c[L];
   unsigned act[L], ahead[L];
@@ -275,9 +287,13 @@ __global__ __launch_bounds__(kThreads, S > 1 ? 4 : 1) void scan_fwd_kernel(ScanA
     }
     if constexpr (!MAPS) {
       T* out = static_cast<T*>(p.h) + at.n * p.h_n + at.c;
+      constexpr int GROUP = kGroup<S == 1>;
+      static_assert(L % GROUP == 0, "a group begins with a thread's steps or inside them");
 #pragma unroll
       for (int i = 0; i < L; ++i) {
         const int64_t t = t0 + strand * L + i;
+        if (i % GROUP == 0 && p.states && at.there && t > 0 && t < t_end)
+          put<TINY>(p.states + ((t / GROUP - 1) * p.N + at.n) * p.H + at.c, at.left, start);
 #pragma unroll
         for (int k = 0; k < 4; ++k) start[k] = __builtin_fmaf(a[i][k], start[k], b[i][k]);
         if (at.there && t < t_end) put<TINY>(out + t * p.h_t, at.left, start);
@@ -302,10 +318,11 @@ __global__ __launch_bounds__(kThreads, S > 1 ? 4 : 1) void scan_fwd_kernel(ScanA
 }
 
 // Backward, from the last step down: strand 0 has the latest steps of a tile, split 0 the latest
-// steps of all.
+// steps of all.  A thread's L steps are a group: they begin at a multiple of L, and the states before each
+// of them come from the one before the group, by the forward pass's own arithmetic.
 template <typename T, int C, int S, bool MAPS, bool TINY>
-__global__ __launch_bounds__(kThreads, S > 1 || sizeof(T) == 2 ? 4 : 1) void scan_bwd_kernel(ScanArgs p) {
-  constexpr int L = S == 1 ? kBwdWalkSteps<T> : kBwdSteps;
+__global__ __launch_bounds__(kThreads, S > 1 ? 4 : 1) void scan_bwd_kernel(ScanArgs p) {
+  constexpr int L = kGroup<S == 1>;
   constexpr bool STREAM = S == 1;
   static_assert(C * S == kThreads, "lanes x strands");
   __shared__ float4 meet[S > 1 ? 2 : 1][S][2][S > 1 ? C : 1];
@@ -314,47 +331,49 @@ __global__ __launch_bounds__(kThreads, S > 1 || sizeof(T) == 2 ? 4 : 1) void sca
   const Place at(p, channel);
   const int split = blockIdx.y;
   const int64_t lanes4 = p.N * p.Hq * 4;
-  // steps counted from the end: u = T - 1 - t
+  // steps counted from the end of the last group: u = groups L - 1 - t
+  const int64_t steps = (p.T + L - 1) / L * L;
   const int64_t u_begin = split * p.per_split;
-  const int64_t u_end = u_begin + p.per_split < p.T ? u_begin + p.per_split : p.T;
+  const int64_t u_end = u_begin + p.per_split < steps ? u_begin + p.per_split : steps;
   const T* gates = static_cast<const T*>(p.gates) + at.n * p.gates_n + at.c;
   const T* g = static_cast<const T*>(p.g) + (p.g ? at.n * p.g_n + at.c : 0);
-  const T* h = static_cast<const T*>(p.h) + at.n * p.h_n + at.c;
   const uint8_t* active = p.active ? p.active + at.n * p.active_n : nullptr;
+  const float* const h0 = p.h0 ? p.h0 + at.n * p.h0_n + at.c : nullptr;
+  const float* const before = p.before ? p.before + at.n * p.before_n + at.c : nullptr;
 
-  held<T> raw_z[L], raw_c[L], raw_g[L], raw_h[L];
+  held<T> raw_z[L], raw_c[L], raw_g[L];
+  held<float> raw_s;
   unsigned act[L], ahead[L];
+  // The step at u, kept among those of the split: steps that are not there read a neighbour again.
+  auto step_at = [&](int64_t u) {
+    const int64_t t = steps - 1 - (u < u_end ? u : u_end - 1);
+    return t < p.T ? t : p.T - 1;
+  };
   auto look = [&](int64_t u0) {
     if (active) {
 #pragma unroll
-      for (int i = 0; i < L; ++i) {
-        const int64_t u = u0 + strand * L + i;
-        ahead[i] = active[(p.T - 1 - (u < u_end ? u : u_end - 1)) * p.active_t];
-      }
+      for (int i = 0; i < L; ++i) ahead[i] = active[step_at(u0 + strand * L + i) * p.active_t];
     }
   };
   auto fetch = [&](int64_t u0) {
 #pragma unroll
     for (int i = 0; i < L; ++i) {
-      int64_t u = u0 + strand * L + i;
-      u = u < u_end ? u : u_end - 1;
-      const int64_t t = p.T - 1 - u;
+      const int64_t t = step_at(u0 + strand * L + i);
       if constexpr (S == 1) act[i] = active ? ahead[i] : 1u;
       if (S > 1 || act[i]) {
         raw_z[i] = take<STREAM, TINY>(gates + t * p.gates_t, at.left);
-        if constexpr (!MAPS) {
-          raw_c[i] = take<STREAM, TINY>(gates + t * p.gates_t + p.H, at.left);
-          // the state before the step; before the first one it is h0, put in below
-          raw_h[i] = take<STREAM, TINY>(h + (t > 0 ? t - 1 : 0) * p.h_t, at.left);
-        }
+        if constexpr (!MAPS) raw_c[i] = take<STREAM, TINY>(gates + t * p.gates_t + p.H, at.left);
       }
     }
     if (p.g) {
 #pragma unroll
-      for (int i = 0; i < L; ++i) {
-        const int64_t u = u0 + strand * L + i;
-        raw_g[i] = take<STREAM, TINY>(g + (p.T - 1 - (u < u_end ? u : u_end - 1)) * p.g_t, at.left);
-      }
+      for (int i = 0; i < L; ++i) raw_g[i] = take<STREAM, TINY>(g + step_at(u0 + strand * L + i) * p.g_t, at.left);
+    }
+    if constexpr (!MAPS) {
+      const int64_t group = (steps - 1 - (u0 + strand * L)) / L;  // strands past the end: not above zero
+      const float* const src = group > 0 ? before + (group - 1) * p.before_g : h0;
+      raw_s = held<float>{0.0f, 0.0f, 0.0f, 0.0f};
+      if (src) raw_s = take<STREAM, TINY>(src, at.left);
     }
     look(S == 1 ? u0 + L : u0);
     if constexpr (S > 1) {
@@ -404,26 +423,31 @@ __global__ __launch_bounds__(kThreads, S > 1 || sizeof(T) == 2 ? 4 : 1) void sca
   for (int64_t u0 = u_begin; u0 < u_end; u0 += S * L) {
     if (S > 1 && u0 != u_begin) fetch(u0);
     float a[L][4], rest[L][4], gv[L][4], away[L][4];  // away: the state before the step, less c
-    bool on[L];
+    bool there[L], on[L];
 #pragma unroll
     for (int i = 0; i < L; ++i) {
       const int64_t u = u0 + strand * L + i;
-      on[i] = u < u_end && act[i] != 0;
+      there[i] = u < u_end && steps - 1 - u < p.T;
+      on[i] = there[i] && act[i] != 0;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         gate_pair(on[i] ? widen(raw_z[i][k]) : __builtin_inff(), a[i][k], rest[i][k]);  // 1, 0 for a step passed over
         // a step that is not there passes e on as it is
-        gv[i][k] = p.g && u < u_end ? widen(raw_g[i][k]) : 0.0f;
-        if constexpr (!MAPS) away[i][k] = widen(raw_h[i][k]) - widen(raw_c[i][k]);
+        gv[i][k] = p.g && there[i] ? widen(raw_g[i][k]) : 0.0f;
       }
-      if constexpr (!MAPS) {
-        if (u == p.T - 1) {
-          float before[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          if (p.h0) load4_upto(p.h0 + at.n * p.h0_n + at.c, at.left, 0.0f, before);
+    }
+    if constexpr (!MAPS) {
+      float state[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) away[i][k] = before[k] - widen(raw_c[i][k]);
+      for (int k = 0; k < 4; ++k) state[k] = raw_s[k];
+#pragma unroll
+      for (int i = L - 1; i >= 0; --i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float c = on[i] ? widen(raw_c[i][k]) : 0.0f;
+          away[i][k] = state[k] - c;
+          state[k] = __builtin_fmaf(a[i][k], state[k], rest[i][k] * c);
         }
-      }
     }
     if (S == 1 && u0 + L < u_end) fetch(u0 + L);
     float start[4];
@@ -461,7 +485,7 @@ __global__ __launch_bounds__(kThreads, S > 1 || sizeof(T) == 2 ? 4 : 1) void sca
       T* out = static_cast<T*>(p.dgates) + at.n * p.dg_n + at.c;
 #pragma unroll
       for (int i = 0; i < L; ++i) {
-        const int64_t u = u0 + strand * L + i, t = p.T - 1 - u;
+        const int64_t u = u0 + strand * L + i, t = steps - 1 - u;
         float dz[4], dc[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -470,7 +494,7 @@ __global__ __launch_bounds__(kThreads, S > 1 || sizeof(T) == 2 ? 4 : 1) void sca
           dz[k] = on[i] ? d * away[i][k] * (a[i][k] * rest[i][k]) : 0.0f;
           start[k] = a[i][k] * d;
         }
-        if (p.dgates && at.there && u < u_end) {
+        if (p.dgates && at.there && there[i]) {
           put<TINY>(out + t * p.dg_t, at.left, dz);
           put<TINY>(out + t * p.dg_t + p.H, at.left, dc);
         }
@@ -512,6 +536,7 @@ Plan plan_for(int64_t T, int64_t N, int64_t H, int steps) {
   const int64_t per = (tiles + splits - 1) / splits * tile;
   return {false, static_cast<int>((T + per - 1) / per), per};
 }
+int64_t group_of(const Plan& q) { return q.walk ? kGroup<true> : kGroup<false>; }
 size_t maps_bytes(int64_t T, int64_t N, int64_t H, int steps) {
   const Plan q = plan_for(T, N, H, steps);
   return q.splits > 1 ? static_cast<size_t>(q.splits) * 2 * N * ((H + 3) / 4) * 4 * sizeof(float) : 0;
@@ -643,9 +668,14 @@ size_t spmi_gated_scan_bwd_workspace_bytes(int64_t T, int64_t N, int64_t H) {
   return T > 0 && N > 0 && H > 0 ? maps_bytes(T, N, H, kBwdSteps) : 0;
 }
 
-int spmi_gated_scan_fwd(const void* gates, int dtype, int64_t gates_t, int64_t gates_n, const float* h0, int64_t h0_n,
-                        const uint8_t* active, int64_t active_t, int64_t active_n, int64_t T, int64_t N, int64_t H,
-                        void* h, int64_t h_t, int64_t h_n, float* last, void* ws, size_t ws_bytes, void* stream) {
+int64_t spmi_gated_scan_states(int64_t T, int64_t N, int64_t H) {
+  return T > 0 && N > 0 && H > 0 ? (T - 1) / group_of(plan_for(T, N, H, kBwdSteps)) : 0;
+}
+
+int spmi_gated_scan_fwd_saved(const void* gates, int dtype, int64_t gates_t, int64_t gates_n, const float* h0,
+                              int64_t h0_n, const uint8_t* active, int64_t active_t, int64_t active_n, int64_t T,
+                              int64_t N, int64_t H, void* h, int64_t h_t, int64_t h_n, float* last, float* states,
+                              void* ws, size_t ws_bytes, void* stream) {
   if (int rc = check_sizes("spmi_gated_scan_fwd", dtype, T, N, H)) return rc;
   if (N == 0) return SPMI_OK;
   SPMI_REQUIRE(last && (T == 0 || (gates && h)), SPMI_ERR_INVALID_ARG, "spmi_gated_scan_fwd: null pointer");
@@ -658,7 +688,7 @@ int spmi_gated_scan_fwd(const void* gates, int dtype, int64_t gates_t, int64_t g
   a.gates = gates; a.gates_t = gates_t; a.gates_n = gates_n;
   a.h0 = h0; a.h0_n = h0_n;
   a.active = active; a.active_t = active_t; a.active_n = active_n;
-  a.h = h; a.h_t = h_t; a.h_n = h_n; a.last = last;
+  a.h = h; a.h_t = h_t; a.h_n = h_n; a.last = last; a.states = states;
   a.T = T; a.N = N; a.H = static_cast<int>(H); a.Hq = static_cast<int>((H + 3) / 4);
   a.per_split = q.per_split; a.splits = q.splits; a.maps = static_cast<float*>(ws);
   const bool tiny = H < 4;
@@ -668,15 +698,25 @@ int spmi_gated_scan_fwd(const void* gates, int dtype, int64_t gates_t, int64_t g
   return SPMI_OK;
 }
 
+int spmi_gated_scan_fwd(const void* gates, int dtype, int64_t gates_t, int64_t gates_n, const float* h0, int64_t h0_n,
+                        const uint8_t* active, int64_t active_t, int64_t active_n, int64_t T, int64_t N, int64_t H,
+                        void* h, int64_t h_t, int64_t h_n, float* last, void* ws, size_t ws_bytes, void* stream) {
+  return spmi_gated_scan_fwd_saved(gates, dtype, gates_t, gates_n, h0, h0_n, active, active_t, active_n, T, N, H, h,
+                                   h_t, h_n, last, nullptr, ws, ws_bytes, stream);
+}
+
 int spmi_gated_scan_bwd(const void* gates, int dtype, int64_t gates_t, int64_t gates_n, const float* h0, int64_t h0_n,
                         const uint8_t* active, int64_t active_t, int64_t active_n, int64_t T, int64_t N, int64_t H,
-                        const void* h, int64_t h_t, int64_t h_n, const void* g, int64_t g_t, int64_t g_n,
-                        const float* g_last, int64_t gl_n, void* dgates, int64_t dg_t, int64_t dg_n, float* dh0,
+                        const void* h, int64_t h_t, int64_t h_n, const float* states, const void* g, int64_t g_t,
+                        int64_t g_n, const float* g_last, int64_t gl_n, void* dgates, int64_t dg_t, int64_t dg_n, float* dh0,
                         void* ws, size_t ws_bytes, void* stream) {
   if (int rc = check_sizes("spmi_gated_scan_bwd", dtype, T, N, H)) return rc;
   if (N == 0 || (T == 0 && !dh0)) return SPMI_OK;
-  SPMI_REQUIRE((T == 0 || gates) && (T <= 1 || h), SPMI_ERR_INVALID_ARG, "spmi_gated_scan_bwd: null pointer");
+  const bool f32 = dtype == SPMI_DTYPE_F32;
   const Plan q = plan_for(T, N, H, kBwdSteps);
+  const int64_t group = group_of(q);
+  SPMI_REQUIRE((T == 0 || gates) && (T <= group || (f32 ? h != nullptr : states != nullptr)), SPMI_ERR_INVALID_ARG,
+               "spmi_gated_scan_bwd: null pointer");
   SPMI_REQUIRE(q.splits == 1 || (ws && ws_bytes >= maps_bytes(T, N, H, kBwdSteps)), SPMI_ERR_WORKSPACE,
                "spmi_gated_scan_bwd: workspace of %zu bytes is too small", ws_bytes);
   SPMI_REQUIRE((reinterpret_cast<uintptr_t>(ws) & 15) == 0, SPMI_ERR_INVALID_ARG,
@@ -685,16 +725,18 @@ int spmi_gated_scan_bwd(const void* gates, int dtype, int64_t gates_t, int64_t g
   a.gates = gates; a.gates_t = gates_t; a.gates_n = gates_n;
   a.h0 = h0; a.h0_n = h0_n;
   a.active = active; a.active_t = active_t; a.active_n = active_n;
-  a.h = const_cast<void*>(h); a.h_t = h_t; a.h_n = h_n;
-  if (T == 1) {  // there may be no h: what is read in place of the states before the first step is not used
-    a.h = const_cast<void*>(gates); a.h_t = gates_t; a.h_n = gates_n;
+  if (T > group && f32) {  // float32 states are whole where they stand in h
+    a.before = static_cast<const float*>(h) + (group - 1) * h_t; a.before_g = group * h_t; a.before_n = h_n;
+  } else if (T > group) {
+    a.before = states; a.before_g = N * H; a.before_n = H;
   }
   a.g = g; a.g_t = g_t; a.g_n = g_n; a.g_last = g_last; a.gl_n = gl_n;
   a.dgates = dgates; a.dg_t = dg_t; a.dg_n = dg_n; a.dh0 = dh0;
   a.T = T; a.N = N; a.H = static_cast<int>(H); a.Hq = static_cast<int>((H + 3) / 4);
-  a.per_split = q.per_split; a.splits = q.splits; a.maps = static_cast<float*>(ws);
+  a.per_split = q.walk ? T + group : q.per_split;  // walking: all steps of the last group too
+  a.splits = q.splits; a.maps = static_cast<float*>(ws);
   const bool tiny = H < 4;
-  if (dtype == SPMI_DTYPE_F32) (tiny ? launch_bwd<float, true> : launch_bwd<float, false>)(a, q, as_stream(stream));
+  if (f32) (tiny ? launch_bwd<float, true> : launch_bwd<float, false>)(a, q, as_stream(stream));
   else (tiny ? launch_bwd<bf16, true> : launch_bwd<bf16, false>)(a, q, as_stream(stream));
   SPMI_CHECK_LAUNCH("spmi_gated_scan_bwd");
   return SPMI_OK;
