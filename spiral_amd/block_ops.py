@@ -14,7 +14,6 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as nv
 from .graph import _ACT_CODES
@@ -92,19 +91,46 @@ def _launch(name: str, at: int, *args) -> None:
         nv.check(rc, name)
 
 
+class _OnceOnly(torch.autograd.Function):
+    """Gradients as they are, in a graph that leads back to `anchors` and cannot be walked."""
+
+    @staticmethod
+    def forward(ctx, name, anchors, *values):
+        ctx.name = name
+        return tuple(v.detach() for v in values[anchors:])
+
+    @staticmethod
+    def backward(ctx, *g):
+        _refuse(f"{ctx.name} has no second derivative")
+
+
 class _Operator(torch.autograd.Function):
     """Base of the operators below: `gradients(ctx, *g)` is the backward pass.  It runs kernels
-    autograd does not see, so a second derivative through it raises instead of being wrong; the
-    wrapper for that (a few us) is only taken where a graph of the backward pass is recorded."""
+    autograd does not see, so a second derivative through it raises instead of being wrong: where a
+    graph of the backward pass is recorded, its results depend on whatever they were computed
+    from, the saved inputs as well as the incoming gradients, through a node that raises."""
 
     @staticmethod
     def gradients(ctx, *g):
         raise NotImplementedError
 
     @classmethod
-    def _bind(cls):
-        plain, once = cls.gradients, once_differentiable(cls.gradients)
-        cls.backward = staticmethod(lambda ctx, *g: once(ctx, *g) if _tracking() else plain(ctx, *g))
+    def _bind(cls, name):
+        plain = cls.gradients
+
+        def backward(ctx, *g):
+            if not _tracking():
+                return plain(ctx, *g)
+            with torch.no_grad():
+                found = list(plain(ctx, *g))
+            anchors = [t for t in (*ctx.saved_tensors, *g) if t is not None and t.requires_grad]
+            at = [i for i, t in enumerate(found) if t is not None]
+            if anchors and at:
+                for i, t in zip(at, _OnceOnly.apply(name, len(anchors), *anchors, *(found[i] for i in at))):
+                    found[i] = t
+            return tuple(found)
+
+        cls.backward = staticmethod(backward)
         return cls
 
 
@@ -161,7 +187,7 @@ class _LayerNorm(_Operator):
         return dx, dw, db, None, None, None
 
 
-_LayerNorm._bind()
+_LayerNorm._bind("layer_norm")
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -259,7 +285,7 @@ class _GatedScan(_Operator):
         return dgates, dh0, None, None, None, None
 
 
-_GatedScan._bind()
+_GatedScan._bind("gated_scan")
 
 
 def gated_scan(gates: torch.Tensor, h0: Optional[torch.Tensor] = None, active: Optional[torch.Tensor] = None,
@@ -327,7 +353,7 @@ class _GatedStep(_Operator):
         return dgates, None, None, None, None, None
 
 
-_GatedStep._bind()
+_GatedStep._bind("gated_step")
 
 
 def gated_step(gates: torch.Tensor, h_mem: torch.Tensor, ids: Optional[torch.Tensor] = None,

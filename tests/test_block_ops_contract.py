@@ -27,3 +27,31 @@ def test_states_kept_for_the_backward_pass():
     assert lib.spmi_gated_scan_fwd_saved(P, 0, 8, 8, None, 0, None, 0, 0, 1, 1, 4, P, 4, 4, None, P, None, 0, None) == -1
     with pytest.raises(nv.SpmiError):
         ops.gated_scan(torch.zeros(3, 2, 8, dtype=torch.bfloat16))
+
+
+def test_a_second_derivative_is_refused_whatever_the_incoming_gradient():
+    """The base of the operators on the CPU, with x^2 in the place of a kernel: at x = 3 the derivative of
+    x + (dx^2/dx)^2 is 1 + 8 x = 25; taking the backward pass' result for a constant would give 1."""
+    from spiral_amd.block_ops import _Operator
+
+    class Square(_Operator):
+        @staticmethod
+        def forward(ctx, x, y):
+            ctx.save_for_backward(x)
+            return x * x
+
+        @staticmethod
+        def gradients(ctx, g):
+            return 2 * ctx.saved_tensors[0] * g, None
+
+    Square._bind("square")
+    x = torch.tensor(3.0, requires_grad=True)
+    y = Square.apply(x, None)
+    (dx,) = torch.autograd.grad(y, x, create_graph=True)
+    assert float(dx.detach()) == 6.0 and dx.requires_grad
+    with pytest.raises(nv.SpmiError, match="square has no second derivative"):
+        torch.autograd.grad(x + dx.square(), x)
+    g = torch.ones((), requires_grad=True)
+    (dx,) = torch.autograd.grad(Square.apply(x, None), x, g, create_graph=True)
+    with pytest.raises(nv.SpmiError, match="second derivative"):
+        dx.backward()

@@ -1,0 +1,60 @@
+"""What autograd may and may not do with layer norm, the gated linear recurrence and the 8-bit
+projection."""
+import pytest
+import torch
+
+from spiral_amd import _native as nv
+from spiral_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def rand(*shape, seed=0):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return torch.randn(*shape, generator=g, device="cuda")
+
+
+def cases():
+    w, b = rand(12, seed=1), rand(12, seed=2)
+    h0 = rand(3, 4, seed=3)
+    yield "layer_norm", lambda x: ops.layer_norm(x, w, b), rand(5, 12)
+    yield "layer_norm", lambda x: ops.layer_norm(rand(5, 12), x, b), w
+    for dtype in (torch.float32, torch.bfloat16):
+        gates = rand(6, 3, 8, seed=4).to(dtype)
+        yield "gated_scan", lambda x: ops.gated_scan(x, h0)[0], gates
+        yield "gated_scan", lambda x: ops.gated_scan(x, h0)[1], gates
+    yield "gated_step", lambda x: ops.gated_step(x, h0.clone()), rand(3, 8, seed=5)
+
+
+@pytest.mark.parametrize("which", range(7))
+def test_second_derivatives_are_refused(dev, which):
+    name, f, at = list(cases())[which]
+    x = at.clone().requires_grad_()
+    (want,) = torch.autograd.grad(f(x).sum(), x)
+    (dx,) = torch.autograd.grad(f(x).sum(), x, create_graph=True)  # an incoming gradient of constants
+    assert torch.equal(dx, want)
+    with pytest.raises(nv.SpmiError, match=f"{name} has no second derivative"):
+        (x.sum() + dx.float().square().sum()).backward()
+
+
+def test_gradients_of_one_input_move_with_another(dev):
+    """The weight's gradient depends on x, the gates' on h0: neither comes out as a constant."""
+    x, w = rand(5, 12).requires_grad_(), rand(12, seed=1).requires_grad_()
+    (dw,) = torch.autograd.grad(ops.layer_norm(x, w).sum(), w, create_graph=True)
+    with pytest.raises(nv.SpmiError, match="second derivative"):
+        torch.autograd.grad(dw.square().sum(), x)
+    gates, h0 = rand(6, 3, 8).requires_grad_(), rand(3, 4, seed=1).requires_grad_()
+    (dg,) = torch.autograd.grad(ops.gated_scan(gates, h0)[0].sum(), gates, create_graph=True)
+    with pytest.raises(nv.SpmiError, match="second derivative"):
+        torch.autograd.grad(dg.square().sum(), h0)
+
+
+def test_a_recorded_backward_pass_is_an_ordinary_gradient(dev):
+    x, w = rand(40, 12).requires_grad_(), rand(12, seed=1).requires_grad_()
+    ops.layer_norm(x, w).sum().backward()
+    want = x.grad, w.grad
+    x.grad = w.grad = None
+    ops.layer_norm(x, w).sum().backward(create_graph=True)
+    assert torch.equal(x.grad, want[0]) and torch.equal(w.grad, want[1])
+    x.grad = w.grad = None
