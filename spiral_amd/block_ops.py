@@ -14,6 +14,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nv
 from .graph import _ACT_CODES
@@ -51,6 +52,15 @@ def _device_of(t: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
         nv.require_cuda(t, *others)
         _refuse(f"tensors on different devices: {[str(o.device) for o in (t, *others) if o is not None]}")
     return at
+
+
+def _no_tangent(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuse inputs of forward-mode differentiation: the kernels know nothing of a tangent and would
+    drop it.  Outside a dual level, which is nearly always, this is one comparison."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                _refuse(f"{what} has no forward-mode derivative")
 
 
 def _rows_of(t: torch.Tensor) -> torch.Tensor:
@@ -209,6 +219,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     eps = float(eps)
     if not 0.0 <= eps < float("inf"):
         _refuse(f"layer_norm: eps must be finite and not negative, got {eps}")
+    _no_tangent("layer_norm", x, weight, bias)
     at = _device_of(x, weight, bias)
     if grad and _tracking():
         return _LayerNorm.apply(x, weight, bias, eps, code, at)
@@ -312,6 +323,7 @@ def gated_scan(gates: torch.Tensor, h0: Optional[torch.Tensor] = None, active: O
         grad = grad or h0.requires_grad
     if active is not None and (active.dtype != torch.bool or active.shape != gates.shape[:2]):
         _refuse(f"gated_scan: active must be bool {tuple(gates.shape[:2])}, got {active.dtype} {tuple(active.shape)}")
+    _no_tangent("gated_scan", gates, h0)
     at = _device_of(gates, h0, active)
     if grad and _tracking():
         return _GatedScan.apply(gates, h0, active, batch_first, code, at)
@@ -383,6 +395,7 @@ def gated_step(gates: torch.Tensor, h_mem: torch.Tensor, ids: Optional[torch.Ten
         _refuse(f"gated_step: ids must be int64 [{m}], got {ids.dtype} {tuple(ids.shape)}")
     elif not ids.is_contiguous():
         ids = ids.contiguous()
+    _no_tangent("gated_step", gates, h_mem)
     at = _device_of(gates, h_mem, ids)
     mem_write = bool(mem_write)
     if gates.requires_grad and _tracking():
@@ -400,6 +413,7 @@ def quantize_rows_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     code = _code(x, "quantize_rows_int8: x")
     if x.dim() < 1 or not 1 <= x.shape[-1] <= INT8_MAX_INNER:
         _refuse(f"quantize_rows_int8: the last dimension of x must be 1 to {INT8_MAX_INNER}, got {tuple(x.shape)}")
+    _no_tangent("quantize_rows_int8", x)
     at = _device_of(x)
     xr = _rows_of(x)
     m, k = xr.shape
@@ -444,6 +458,7 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         _refuse("linear_int8: out_dtype must be float32 or bfloat16")
     if grad and _tracking():
         _refuse("linear_int8 has no backward pass: call it under torch.no_grad()")
+    _no_tangent("linear_int8", x, weight_scale, bias)
     at = _device_of(x, weight, weight_scale, bias)
     bias = _float_vector(bias)
     xr, w, s = _rows_of(x), _units_last(weight), _float_vector(weight_scale)

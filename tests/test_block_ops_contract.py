@@ -55,3 +55,36 @@ def test_a_second_derivative_is_refused_whatever_the_incoming_gradient():
     (dx,) = torch.autograd.grad(Square.apply(x, None), x, g, create_graph=True)
     with pytest.raises(nv.SpmiError, match="second derivative"):
         dx.backward()
+
+
+F = torch.zeros
+
+
+@pytest.mark.parametrize("name,call", [
+    ("layer_norm", lambda d: ops.layer_norm(d(F(3, 4)))),
+    ("layer_norm", lambda d: ops.layer_norm(F(3, 4), d(F(4)))),
+    ("layer_norm", lambda d: ops.layer_norm(F(3, 4), None, d(F(4)))),
+    ("gated_scan", lambda d: ops.gated_scan(d(F(3, 2, 8)))),
+    ("gated_scan", lambda d: ops.gated_scan(F(3, 2, 8), d(F(2, 4)))),
+    ("gated_step", lambda d: ops.gated_step(d(F(3, 8)), F(5, 4))),
+    ("gated_step", lambda d: ops.gated_step(F(3, 8), d(F(5, 4)))),
+    ("quantize_rows_int8", lambda d: ops.quantize_rows_int8(d(F(3, 4)))),
+    ("linear_int8", lambda d: ops.linear_int8(d(F(3, 4)), F(5, 4, dtype=torch.int8), F(5))),
+    ("linear_int8", lambda d: ops.linear_int8(F(3, 4), F(5, 4, dtype=torch.int8), d(F(5)))),
+    ("linear_int8", lambda d: ops.linear_int8(F(3, 4), F(5, 4, dtype=torch.int8), F(5), d(F(5)))),
+])
+def test_a_forward_mode_derivative_is_refused(name, call):
+    """A dual tensor does not require a gradient; its tangent must not get lost all the same."""
+    fwd = torch.autograd.forward_ad
+    with fwd.dual_level(), pytest.raises(nv.SpmiError, match=f"{name} has no forward-mode derivative"):
+        call(lambda t: fwd.make_dual(t, torch.ones_like(t)))
+    with fwd.dual_level(), torch.no_grad(), pytest.raises(nv.SpmiError, match="forward-mode"):
+        call(lambda t: fwd.make_dual(t, torch.ones_like(t)))
+    with fwd.dual_level(), pytest.raises(nv.SpmiError, match="GPU"):  # no tangent: the usual answer to a CPU tensor
+        call(lambda t: t)
+
+
+def test_forward_mode_through_the_function_transforms_is_refused():
+    x = torch.ones(3, 4)
+    with pytest.raises(nv.SpmiError, match="forward-mode"):
+        torch.func.jvp(ops.layer_norm, (x,), (x,))
