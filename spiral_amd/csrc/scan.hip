@@ -40,12 +40,12 @@ using namespace spmi;
 
 constexpr int kThreads = 256;
 // Steps a thread holds in registers.  Walking, the loads of the next steps are sent before the stores of
-// the present ones: 32 x 50000 x 128 takes 481 us forward and 1279 trained in float32, 238 and 670 in
+// the present ones: 32 x 50000 x 128 takes 481 us forward and 1253 trained in float32, 238 and 668 in
 // bfloat16 (with 2 steps backward 1319 and 767; forward in float32 without the loads ahead 494, with 2
 // steps 488).  As one of the strands, other waves cover the wait better than registers do (1185 x 2255 x 30
-// trained in bfloat16 takes 475 us with four waves to a SIMD; with six the registers spill, 1.4 times as
+// trained in bfloat16 takes 482 us with four waves to a SIMD; with six the registers spill, 1.4 times as
 // long), and more steps pay less than they cost: 65536 x 1 x 128 42 us with 2 forward, 49 with 4;
-// 1601 x 717 x 64 trained in float32 663 with 2 backward, 1.2 times as long with 4.
+// 1601 x 717 x 64 trained in float32 667 with 2 backward, 1.2 times as long with 4.
 constexpr int kFwdSteps = 2;
 constexpr int kFwdWalkSteps = 4;
 constexpr int kBwdSteps = 2;
@@ -61,7 +61,7 @@ constexpr int64_t kManyLanes = 65536;
 constexpr int64_t kFewSteps = 16;
 // Workgroups from which the steps are not split: two per CU (852 x 221 x 448 in bfloat16, 774 workgroups, takes
 // 139 us unsplit and 188 in two, which read the gates twice).  Below, as many splits as make kTargetGroups
-// (1601 x 717 x 64, 359 workgroups, trained in bfloat16 404 us in five, a sixth longer in two).
+// (1601 x 717 x 64, 359 workgroups, trained in bfloat16 410 us in five, a sixth longer in two).
 constexpr int64_t kEnoughGroups = 512;
 constexpr int64_t kTargetGroups = 2048;
 constexpr int64_t kMaxSplits = 512;
@@ -164,7 +164,7 @@ __global__ __launch_bounds__(kThreads, S > 1 ? 4 : 1) void scan_fwd_kernel(ScanA
   // The loads of all steps are in flight together: steps past the end read the last one again, lanes past
   // the end the first node's; `on` says what counts.  Walking, a thread knows a tile ahead which steps are
   // active (`ahead`) and leaves out the rows of the others without a wait: 32 x 50000 x 128 with about a quarter
-  // of them inactive, trained in float32, 1105 us instead of 1279.  As a strand it reads them (852 x 221 x 448
+  // of them inactive, trained in float32, 1097 us instead of 1253 (in bfloat16 602 and 668).  As a strand it reads them (852 x 221 x 448
   // in bfloat16, ragged: 144 us, with the questions between the loads 171).
   held<T> raw_z[L], raw_c[L];
   unsigned act[L], ahead[L];
@@ -321,6 +321,11 @@ __global__ __launch_bounds__(kThreads, S > 1 ? 4 : 1) void scan_fwd_kernel(ScanA
 // Backward, from the last step down: strand 0 has the latest steps of a tile, split 0 the latest
 // steps of all.  A thread's L steps are a group: they begin at a multiple of L, and the states before each
 // of them come from the one before the group, by the forward pass's own arithmetic.
+//
+// Walking, the bfloat16 form takes 168 registers, which leaves room for three waves to a SIMD: what is the same for
+// all steps of a tile (the address of the state before it) is therefore made again and not kept, and which steps
+// are active is kept in scalar masks.  With 176 registers and two waves, 32 x 50000 x 128 with a quarter
+// of the steps inactive takes 659 us trained, not 602.
 template <typename T, int C, int S, bool MAPS, bool TINY>
 __global__ __launch_bounds__(kThreads, S > 1 ? 4 : 1) void scan_bwd_kernel(ScanArgs p) {
   constexpr int L = kGroup<S == 1>;
@@ -339,12 +344,11 @@ __global__ __launch_bounds__(kThreads, S > 1 ? 4 : 1) void scan_bwd_kernel(ScanA
   const T* gates = static_cast<const T*>(p.gates) + at.n * p.gates_n + at.c;
   const T* g = static_cast<const T*>(p.g) + (p.g ? at.n * p.g_n + at.c : 0);
   const uint8_t* active = p.active ? p.active + at.n * p.active_n : nullptr;
-  const float* const h0 = p.h0 ? p.h0 + at.n * p.h0_n + at.c : nullptr;
-  const float* const before = p.before ? p.before + at.n * p.before_n + at.c : nullptr;
 
   held<T> raw_z[L], raw_c[L], raw_g[L];
   held<float> raw_s;
-  unsigned act[L], ahead[L];
+  unsigned ahead[L];
+  bool act[L];
   // The step at u, kept among those of the split: steps that are not there read a neighbour again.
   auto step_at = [&](int64_t u) {
     const int64_t t = steps - 1 - (u < u_end ? u : u_end - 1);
@@ -360,7 +364,7 @@ __global__ __launch_bounds__(kThreads, S > 1 ? 4 : 1) void scan_bwd_kernel(ScanA
 #pragma unroll
     for (int i = 0; i < L; ++i) {
       const int64_t t = step_at(u0 + strand * L + i);
-      if constexpr (S == 1) act[i] = active ? ahead[i] : 1u;
+      if constexpr (S == 1) act[i] = !active || ahead[i] != 0;
       if (S > 1 || act[i]) {
         raw_z[i] = take<STREAM, TINY>(gates + t * p.gates_t, at.left);
         if constexpr (!MAPS) raw_c[i] = take<STREAM, TINY>(gates + t * p.gates_t + p.H, at.left);
@@ -372,14 +376,14 @@ __global__ __launch_bounds__(kThreads, S > 1 ? 4 : 1) void scan_bwd_kernel(ScanA
     }
     if constexpr (!MAPS) {
       const int64_t group = (steps - 1 - (u0 + strand * L)) / L;  // strands past the end: not above zero
-      const float* const src = group > 0 ? before + (group - 1) * p.before_g : h0;
+      const float* const src = group > 0 ? p.before + (group - 1) * p.before_g : p.h0;
       raw_s = held<float>{0.0f, 0.0f, 0.0f, 0.0f};
-      if (src) raw_s = take<STREAM, TINY>(src, at.left);
+      if (src) raw_s = take<STREAM, TINY>(src + at.n * (group > 0 ? p.before_n : p.h0_n) + at.c, at.left);
     }
     look(S == 1 ? u0 + L : u0);
     if constexpr (S > 1) {
 #pragma unroll
-      for (int i = 0; i < L; ++i) act[i] = active ? ahead[i] : 1u;
+      for (int i = 0; i < L; ++i) act[i] = !active || ahead[i] != 0;
     }
   };
 
@@ -429,7 +433,7 @@ __global__ __launch_bounds__(kThreads, S > 1 ? 4 : 1) void scan_bwd_kernel(ScanA
     for (int i = 0; i < L; ++i) {
       const int64_t u = u0 + strand * L + i;
       there[i] = u < u_end && steps - 1 - u < p.T;
-      on[i] = there[i] && act[i] != 0;
+      on[i] = there[i] && act[i];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         gate_pair(on[i] ? widen(raw_z[i][k]) : __builtin_inff(), a[i][k], rest[i][k]);  // 1, 0 for a step passed over
