@@ -253,14 +253,24 @@ struct Block {
 // are scalars: with addresses of its own a lane would keep two registers for each of its rows.
 //
 // With scales from 2^-127 to 2^121 the product of a sum and both scales can leave float32's range
-// half way although the result lies inside.  Where all scales of the wave are between 2^-60 and
-// 2^60 (`plain`) it cannot; elsewhere it is formed from the scales' significands, and the powers are
-// added and applied at the end.
+// half way although the result lies inside.  Where both scales are between 2^-60 and 2^60 (`is_plain`) it
+// cannot; elsewhere it is formed from the scales' significands, and the powers are added and applied
+// at the end.  Which of the two it is goes by the output's own scales, in every kernel: a result's bits
+// depend neither on its neighbours nor on how many rows there are.  (`plain`: it holds for the whole wave.)
 __device__ __forceinline__ bool is_plain(float s) { return s >= 0x1p-60f && s <= 0x1p60f; }
 
-__device__ __forceinline__ float finish(int acc, float sm, float sn, float bias, int act, float slope) {
+__device__ __forceinline__ float scaled(int acc, float sm, float sn, float bias) {
+  return __builtin_fmaf(static_cast<float>(acc) * sn, sm, bias);
+}
+// The same of any scales; `y` is what `scaled` gives.
+__device__ __forceinline__ float scaled_any(float y, int acc, float sm, float sn, float bias) {
   const float f = static_cast<float>(acc) * __builtin_amdgcn_frexp_mantf(sm) * __builtin_amdgcn_frexp_mantf(sn);
-  const float y = __builtin_amdgcn_ldexpf(f, __builtin_amdgcn_frexp_expf(sm) + __builtin_amdgcn_frexp_expf(sn)) + bias;
+  const float wide = __builtin_amdgcn_ldexpf(f, __builtin_amdgcn_frexp_expf(sm) + __builtin_amdgcn_frexp_expf(sn)) + bias;
+  return is_plain(sm) & is_plain(sn) ? y : wide;  // both at hand: no branch for each output
+}
+
+__device__ __forceinline__ float finish(int acc, float sm, float sn, float bias, int act, float slope) {
+  const float y = scaled_any(scaled(acc, sm, sn, bias), acc, sm, sn, bias);
   if (act == SPMI_ACT_RELU) return y < 0.0f ? 0.0f : y;  // not a maximum: NaN stays
   if (act == SPMI_ACT_LEAKY_RELU) return y < 0.0f ? y * slope : y;
   return y;
@@ -270,12 +280,11 @@ template <typename OUT>
 __device__ __forceinline__ void finish16(const i32x16& acc, const float (&sm)[16], float sn, float bias, bool plain,
                                          int act, float slope, Block<OUT> to, unsigned lane_off, int left) {
   float y[16];
-  if (plain) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) y[r] = __builtin_fmaf(static_cast<float>(acc[r]) * sn, sm[r], bias);
-  } else {
+  for (int r = 0; r < 16; ++r) y[r] = scaled(acc[r], sm[r], sn, bias);
+  if (!plain) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) y[r] = finish(acc[r], sm[r], sn, bias, SPMI_ACT_NONE, 0.0f);
+    for (int r = 0; r < 16; ++r) y[r] = scaled_any(y[r], acc[r], sm[r], sn, bias);
   }
   if (act == SPMI_ACT_RELU) {
 #pragma unroll
@@ -637,6 +646,17 @@ __global__ __launch_bounds__(RowsShape<KP>::NW * 64, 2) void rows_i8_kernel(Rows
     for (int k = 0; k < KS; ++k)
       acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(
           xa[k], *reinterpret_cast<const i32x4*>(slice + lr * SK + k * 32 + lh * 16), acc, 0, 0, 0);
+    if constexpr (KS >= 4) {
+      // Four operands ahead of the products that take them: left to itself the compiler reads each when it is
+      // needed (100003 x 512 -> 1024 takes 157 us so, and 149 with the reads ahead).
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (int k = 0; k < KS - 4; ++k) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+    }
     const float sn = reinterpret_cast<const float*>(slice + 32 * SK)[lr];
     const float bias = reinterpret_cast<const float*>(slice + 32 * SK)[32 + lr];
     const bool all_plain = rows_plain && __all(is_plain(sn));
