@@ -462,12 +462,12 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     at = _device_of(x, weight, weight_scale, bias)
     bias = _float_vector(bias)
     xr, w, s = _rows_of(x), _units_last(weight), _float_vector(weight_scale)
-    if xr.stride(0) >= _INT8_MAX_STRIDE:
-        xr = xr.contiguous()
-    m = xr.shape[0]
+    m, ld = xr.shape[0], xr.stride(0)
+    if ld >= _INT8_MAX_STRIDE:  # of a single row it is the way to nowhere, and torch calls it contiguous
+        xr, ld = xr.contiguous(), k
     out = _empty(*x.shape[:-1], n, dtype=out_dtype, device=x.device)
     ws_bytes = nv.lib().spmi_linear_i8_workspace_bytes(m, k, n)
     ws = _workspace(ws_bytes, x.device)
-    _launch("spmi_linear_i8", at, xr.data_ptr(), code, xr.stride(0), m, k, w.data_ptr(), w.stride(0), s.data_ptr(), n,
+    _launch("spmi_linear_i8", at, xr.data_ptr(), code, ld, m, k, w.data_ptr(), w.stride(0), s.data_ptr(), n,
             _ptr(bias), act_code, slope, out.data_ptr(), out_code, n, _ptr(ws), ws_bytes)
     return out

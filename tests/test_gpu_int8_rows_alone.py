@@ -66,3 +66,15 @@ def test_neighbours_of_channels_out_of_the_ordinary(dev, m, k):
     t = s.clone()
     t[5::33], t[16::33], t[27::33] = 0.0, 1e-30, 1e25
     assert torch.equal(ops.linear_int8(x, w, t, b)[:, ~odd], want[:, ~odd])
+
+
+@pytest.mark.parametrize("m", [0, 1, 2])
+def test_rows_far_apart(dev, m):
+    """Rows 2^24 values and more apart: copied where there are several, and a single one has no distance."""
+    x, w, s, b = problem(2, 128, 40, BF16)
+    wide = torch.zeros(2, 1 << 24, dtype=BF16, device=dev)
+    wide[:, 5:133] = x
+    assert torch.equal(ops.linear_int8(wide[:m, 5:133], w, s, b), ops.linear_int8(x[:m], w, s, b))
+    q, scale = ops.quantize_rows_int8(wide[:m, 5:133])
+    want = ops.quantize_rows_int8(x[:m])
+    assert torch.equal(q, want[0]) and torch.equal(scale, want[1])
