@@ -463,7 +463,7 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     bias = _float_vector(bias)
     xr, w, s = _rows_of(x), _units_last(weight), _float_vector(weight_scale)
     m, ld = xr.shape[0], xr.stride(0)
-    if ld >= _INT8_MAX_STRIDE:  # of a single row it is the way to nowhere, and torch calls it contiguous
+    if ld >= _INT8_MAX_STRIDE:  # a single row's stride says nothing, and torch calls such a view contiguous
         xr, ld = xr.contiguous(), k
     out = _empty(*x.shape[:-1], n, dtype=out_dtype, device=x.device)
     ws_bytes = nv.lib().spmi_linear_i8_workspace_bytes(m, k, n)

@@ -542,7 +542,7 @@ class GLRU(SequentialDecoder):
         for k in range(self.n_layers):
             start = mem.layer(k) if whole else mem.memory[k].index_select(0, ids) if ids is not None \
                 else mem.memory[k][:n].clone()
-            gates = self.base_model.gates(x.reshape(t * n, -1), k).reshape(t, n, 2 * self.hidden_d)
+            gates = self.base_model.gates(x.reshape(t * n, x.shape[2]), k).reshape(t, n, 2 * self.hidden_d)
             x, end = ops.gated_scan(gates, start, active)
             last.append(end.detach())
             x = self._between_layers(x, k)
