@@ -473,8 +473,8 @@ class GatedLinearLayers(nn.Module):
         self.projections = nn.ModuleList(TallLinear(w, 2 * hidden_size, bias=bias) for w in widths)
 
     def gates(self, x: torch.Tensor, k: int) -> torch.Tensor:
-        """[rows, in] -> [rows, 2 * hidden] of layer k."""
-        return self.projections[k](self.norms[k](x))
+        """[rows, in] -> [rows, 2 * hidden] of layer k, in the type of the layer's parameters."""
+        return self.projections[k](self.norms[k](x.to(self.norms[k].weight.dtype)))
 
 
 class GLRU(SequentialDecoder):
@@ -485,7 +485,7 @@ class GLRU(SequentialDecoder):
 
     The gate depends on the input only, so a sequence of snapshots is one scan: `forward_sequence`
     trains through time, where `forward` advances one snapshot from a detached state like GRU, LSTM and
-    RNN.  `to_int8` turns a trained decoder into one that serves with 8-bit projections."""
+    RNN.  Parameters are float32 or bfloat16, the node memory is float32.  `to_int8` turns a trained decoder into one that serves with 8-bit projections."""
 
     _cell_kind = "glru"
 
@@ -495,18 +495,20 @@ class GLRU(SequentialDecoder):
         self.input_d = input_d
         self.base_model = GatedLinearLayers(input_d, hidden_d, n_layers, **kwargs)
 
-    def _rows_in(self, x: torch.Tensor) -> torch.Tensor:
-        return x.to(self.base_model.norms[0].weight.dtype)
+    def _rows_out(self, x: torch.Tensor) -> torch.Tensor:
+        """States for the simple decoder, in the type of its parameters: a step gives float32 states and
+        a scan those of its gates' type, whatever the head is in."""
+        kinds = (p.dtype for p in self.simple_decoder.parameters() if p.is_floating_point())
+        return x.to(next(kinds, x.dtype))
 
     def _step(self, x, ids):
         mem = self.memory_h
-        x = self._rows_in(x)
         for k in range(self.n_layers):
             x = ops.gated_step(self.base_model.gates(x, k), mem.memory[k], ids, mem_write=self.training_mode)
             x = self._between_layers(x, k)
         if self.training_mode:
             mem._bounded = mem._bound_check = None
-        return x
+        return self._rows_out(x)
 
     def forward_sequence(self, node_embs: torch.Tensor, ids: Optional[torch.Tensor] = None,
                          active: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -534,7 +536,7 @@ class GLRU(SequentialDecoder):
             self.memory_h = self.memory_h.to(node_embs.device)
         mem = self.memory_h
         whole = ids is None and n == mem.rows()
-        x = self._rows_in(node_embs)
+        x = node_embs
         if active is not None:
             # a row that is not there must not reach the sums of a weight gradient, not even as 0 * NaN
             x = torch.where(active[..., None], x, torch.zeros((), dtype=x.dtype, device=x.device))
@@ -552,6 +554,7 @@ class GLRU(SequentialDecoder):
             else:
                 mem.update_memory(torch.stack(last), slice(0, n) if ids is None else ids)
             mem._bounded = mem._bound_check = None
+        x = self._rows_out(x)
         if active is not None:
             rows = x[active]
             return self.simple_decoder((rows, torch.arange(rows.shape[0], device=rows.device)))
