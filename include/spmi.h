@@ -695,6 +695,7 @@ int spmi_layer_norm_bwd(const void* x, const void* g, int dtype, int64_t ldx, in
  *   h_t = sigmoid(z) h_{t-1} + (1 - sigmoid(z)) c
  * over T steps for N nodes, as one scan.  gates, h, g, dgates are float32 or bfloat16 (`dtype`)
  * with strides in values along steps (_t) and nodes (_n), units contiguous; states are float32.
+ * H <= 2^24, and the nodes' rows are less than 2^32 - 255 groups of four units (one for each node at least).
  *   h0       nullable (zeros), [N, H] with row stride h0_n
  *   active   nullable, one byte per step and node (strides in bytes): where it is 0 the state
  *            passes unchanged and the gates are not used (their gradient is 0)
@@ -741,7 +742,7 @@ int spmi_gated_step(const void* gates, int dtype, int64_t ldg, float* h_mem, int
  * row of x with a value that is not finite comes out as NaN (its q are 0, its scale NaN).
  * spmi_quantize_rows_i8 gives q and s alone: applied to a weight [N, K] it makes w and w_scale.
  * x and out are float32 or bfloat16; rows of x, w and out have strides in values (of x and out below
- * 2^24) and any alignment.
+ * 2^24) and any alignment; M <= 2^31 - 512.
  * ---------------------------------------------------------------------- */
 int spmi_quantize_rows_i8(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, int8_t* q, int64_t ldq,
                           float* scale, void* stream);

@@ -23,6 +23,8 @@ constexpr int kThreads = 256;
 // The same for LDS: all reads have returned.
 #define WAIT_LDS (15 | (3 << 14) | (7 << 4))
 constexpr int64_t kMaxGroups = 1 << 22;  // of kThreads: a grid holds less than 2^32 threads
+constexpr int64_t kMaxThreads = 1ll << 32;  // of a grid, this not included
+constexpr int64_t kMaxRows = (1ll << 31) - 512;  // with two threads a row (256 rows to a workgroup of 512) below that
 constexpr int64_t kMaxInner = 131072;
 constexpr int64_t kMaxStride = 1 << 24;  // of a row of x and of the output, in values
 // Smallest row maximum that is divided by: 127 / 2^-120 is still finite.
@@ -848,10 +850,10 @@ template <typename OUT, int BM, int BN, int WM, int WN, int ST>
 int launch_tile(const GemmArgs& a, hipStream_t st) {
   constexpr size_t lds = static_cast<size_t>(ST) * (BM + BN) * 64 + (BM + 2 * BN) * sizeof(float);
   const auto kernel = tile_i8_kernel<OUT, BM, BN, WM, WN, ST>;
-  SPMI_RAISE_LDS_LIMIT(kernel, lds);
   const int64_t tiles = ((a.M + BM - 1) / BM) * ((a.N + BN - 1) / BN);
-  SPMI_REQUIRE(tiles < (1ll << 31) - 8, SPMI_ERR_UNSUPPORTED, "spmi_linear_i8: %lld x %lld outputs are too many",
-               (long long)a.M, (long long)a.N);
+  SPMI_REQUIRE((tiles + 7) / 8 * 8 < kMaxThreads / (WM * WN * 64), SPMI_ERR_UNSUPPORTED,
+               "spmi_linear_i8: %lld x %lld outputs are too many", (long long)a.M, (long long)a.N);
+  SPMI_RAISE_LDS_LIMIT(kernel, lds);
   kernel<<<static_cast<unsigned>((tiles + 7) / 8 * 8), WM * WN * 64, lds, st>>>(a);
   return SPMI_OK;
 }
@@ -911,9 +913,9 @@ bool few_made(int64_t M, int64_t K, int64_t N) {
 int check_rows(const char* what, int dtype, int64_t M, int64_t K) {
   SPMI_REQUIRE(dtype == SPMI_DTYPE_F32 || dtype == SPMI_DTYPE_BF16, SPMI_ERR_INVALID_ARG, "%s: dtype %d", what, dtype);
   SPMI_REQUIRE(M >= 0 && K >= 1, SPMI_ERR_INVALID_ARG, "%s: M=%lld K=%lld", what, (long long)M, (long long)K);
-  SPMI_REQUIRE(K <= kMaxInner && M < (1ll << 31), SPMI_ERR_UNSUPPORTED,
-               "%s: %lld rows of %lld values (at most 2^31 - 1 rows of %lld)", what, (long long)M, (long long)K,
-               (long long)kMaxInner);
+  SPMI_REQUIRE(K <= kMaxInner && M <= kMaxRows, SPMI_ERR_UNSUPPORTED,
+               "%s: %lld rows of %lld values (at most %lld rows of %lld)", what, (long long)M, (long long)K,
+               (long long)kMaxRows, (long long)kMaxInner);
   return SPMI_OK;
 }
 

@@ -576,9 +576,9 @@ int check_sizes(const char* what, int dtype, int64_t T, int64_t N, int64_t H) {
   SPMI_REQUIRE(dtype == SPMI_DTYPE_F32 || dtype == SPMI_DTYPE_BF16, SPMI_ERR_INVALID_ARG, "%s: dtype %d", what, dtype);
   SPMI_REQUIRE(T >= 0 && N >= 0 && H >= 1, SPMI_ERR_INVALID_ARG, "%s: T=%lld N=%lld H=%lld", what, (long long)T,
                (long long)N, (long long)H);
-  // a thread for each four units, and a grid holds less than 2^32 threads
-  SPMI_REQUIRE(H <= (1 << 24) && N < (1ll << 33) / H, SPMI_ERR_UNSUPPORTED, "%s: N=%lld H=%lld is too large", what,
-               (long long)N, (long long)H);
+  // a thread for each four units (a row has one at least), and a grid holds less than 2^32 threads
+  SPMI_REQUIRE(H <= (1 << 24) && N <= ((1ll << 32) - kThreads) / ((H + 3) / 4), SPMI_ERR_UNSUPPORTED,
+               "%s: N=%lld H=%lld is too large", what, (long long)N, (long long)H);
   return SPMI_OK;
 }
 

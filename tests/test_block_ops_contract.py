@@ -88,3 +88,15 @@ def test_forward_mode_through_the_function_transforms_is_refused():
     x = torch.ones(3, 4)
     with pytest.raises(nv.SpmiError, match="forward-mode"):
         torch.func.jvp(ops.layer_norm, (x,), (x,))
+
+
+def test_more_threads_than_a_grid_holds_are_refused():
+    """A thread for each four units of a node, one at least; two for each row of the projection."""
+    lib = nv.lib()
+    scan = lib.spmi_gated_scan_fwd
+    for n, h in ((1 << 32, 1), ((1 << 32) - 255, 2), ((1 << 31) - 127, 5)):
+        assert scan(P, 0, 2 * h, 2 * h, None, 0, None, 0, 0, 1, n, h, P, h, h, P, None, 0, None) == -5
+    lin, need = lib.spmi_linear_i8, lib.spmi_linear_i8_workspace_bytes
+    for m in ((1 << 31) - 511, (1 << 31) - 1):
+        assert lin(P, 1, 1, m, 1, P, 1, P, 1, None, 0, 0.0, P, 1, 1, P, need(m, 1, 1), None) == -5
+        assert lib.spmi_quantize_rows_i8(P, 1, 1, m, 1, P, 1, P, None) == -5
