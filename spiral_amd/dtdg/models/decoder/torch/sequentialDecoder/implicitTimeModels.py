@@ -516,16 +516,20 @@ class GLRU(SequentialDecoder):
         every snapshot belonging to node ids[n] (None: node n), `active` bool [T, N] False where a node
         is not in the snapshot: its state passes unchanged, whatever its row holds.  The recurrence
         starts from the node memory (detached) and, in train mode, leaves the last states there;
-        `ids` names each node once.  Returns the simple decoder's output for every row, [T, N, ...],
+        `ids` names each node once; on the host they are looked at, on the GPU an unknown node ends the process
+        in torch's indexing.  Returns the simple decoder's output for every row, [T, N, ...],
         or, with `active`, for the active rows alone (one device round trip for their number) in the
         order of the snapshots: what T calls of `forward` return, one after the other."""
         if node_embs.dim() != 3 or node_embs.shape[2] != self.input_d:
             raise ValueError(f"node_embs must be [T, N, {self.input_d}], got {tuple(node_embs.shape)}")
         t, n, _ = node_embs.shape
         if ids is not None:
-            ids = torch.as_tensor(ids, dtype=torch.int64, device=node_embs.device)
+            ids = torch.as_tensor(ids, dtype=torch.int64)
             if ids.shape != (n,):
                 raise ValueError(f"ids must have one entry for each of the {n} nodes, got {tuple(ids.shape)}")
+            if not ids.is_cuda and n and not (0 <= int(ids.min()) and int(ids.max()) < self.n_nodes):
+                raise ValueError(f"ids must be nodes 0 to {self.n_nodes - 1}, got {int(ids.min())} to {int(ids.max())}")
+            ids = ids.to(node_embs.device)
         elif n > self.n_nodes:
             raise ValueError(f"{n} nodes, but the memory holds {self.n_nodes}")
         if active is not None and (active.dtype != torch.bool or active.shape != (t, n)

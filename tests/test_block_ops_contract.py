@@ -100,3 +100,14 @@ def test_more_threads_than_a_grid_holds_are_refused():
     for m in ((1 << 31) - 511, (1 << 31) - 1):
         assert lin(P, 1, 1, m, 1, P, 1, P, 1, None, 0, 0.0, P, 1, 1, P, need(m, 1, 1), None) == -5
         assert lib.spmi_quantize_rows_i8(P, 1, 1, m, 1, P, 1, P, None) == -5
+
+
+@pytest.mark.parametrize("ids", [[0, 1, 5], [-1, 0, 1], torch.tensor([2, 3, 7])])
+def test_sequences_of_unknown_nodes_are_refused(ids):
+    """torch's indexing on the GPU would end the process."""
+    from spiral_amd.dtdg.models.decoder.sequentialDecoders import GLRU
+    from spiral_amd.dtdg.models.decoder.simpleDecoders import MLP
+
+    dec = GLRU(6, 4, 5, 1, MLP(4, [3]))
+    with pytest.raises(ValueError, match="nodes 0 to 4"):
+        dec.forward_sequence(torch.zeros(2, 3, 6), ids)

@@ -1,5 +1,4 @@
-"""The GLRU decoder at the ends of what it takes: no snapshots, no nodes, one of each; bfloat16 modules;
-unknown nodes."""
+"""The GLRU decoder at the ends of what it takes: no snapshots, no nodes, one of each; bfloat16 modules."""
 import pytest
 import torch
 
