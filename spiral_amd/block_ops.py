@@ -115,13 +115,14 @@ class _OnceOnly(torch.autograd.Function):
 
 
 class _Operator(torch.autograd.Function):
-    """Base of the operators below: `gradients(ctx, *g)` is the backward pass.  It runs kernels
+    """Base of the operators below: `gradients(ctx, saved, *g)` is the backward pass.  It runs kernels
     autograd does not see, so a second derivative through it raises instead of being wrong: where a
     graph of the backward pass is recorded, its results depend on whatever they were computed
-    from, the saved inputs as well as the incoming gradients, through a node that raises."""
+    from, the saved inputs as well as the incoming gradients, through a node that raises.  (The saved
+    tensors are asked for once: activation checkpointing hands them out once.)"""
 
     @staticmethod
-    def gradients(ctx, *g):
+    def gradients(ctx, saved, *g):
         raise NotImplementedError
 
     @classmethod
@@ -129,11 +130,12 @@ class _Operator(torch.autograd.Function):
         plain = cls.gradients
 
         def backward(ctx, *g):
+            saved = ctx.saved_tensors
             if not _tracking():
-                return plain(ctx, *g)
+                return plain(ctx, saved, *g)
             with torch.no_grad():
-                found = list(plain(ctx, *g))
-            anchors = [t for t in (*ctx.saved_tensors, *g) if t is not None and t.requires_grad]
+                found = list(plain(ctx, saved, *g))
+            anchors = [t for t in (*saved, *g) if t is not None and t.requires_grad]
             at = [i for i, t in enumerate(found) if t is not None]
             if anchors and at:
                 for i, t in zip(at, _OnceOnly.apply(name, len(anchors), *anchors, *(found[i] for i in at))):
@@ -168,8 +170,8 @@ class _LayerNorm(_Operator):
         return y
 
     @staticmethod
-    def gradients(ctx, g):
-        x, weight, stats = ctx.saved_tensors
+    def gradients(ctx, saved, g):
+        x, weight, stats = saved
         code, at, m, d, ld, ws_bytes, bias_dtype = ctx.plain
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dev = x.device
@@ -280,8 +282,8 @@ class _GatedScan(_Operator):
         return h, last
 
     @staticmethod
-    def gradients(ctx, g, g_last):
-        gates, h0, active, h, states = ctx.saved_tensors
+    def gradients(ctx, saved, g, g_last):
+        gates, h0, active, h, states = saved
         batch_first, code, at, sizes, ws_bytes = ctx.plain
         need_gates, need_h0 = ctx.needs_input_grad[:2]
         if g is None and g_last is None:
@@ -354,9 +356,9 @@ class _GatedStep(_Operator):
         return h
 
     @staticmethod
-    def gradients(ctx, g):
+    def gradients(ctx, saved, g):
         # the scan's backward pass over one step, with the rows' old states as its start
-        gates, before = ctx.saved_tensors
+        gates, before = saved
         gates = _units_last(gates)
         dgates = _empty(gates.shape, dtype=gates.dtype, device=gates.device)
         m, h2 = gates.shape

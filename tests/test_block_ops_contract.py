@@ -41,8 +41,8 @@ def test_a_second_derivative_is_refused_whatever_the_incoming_gradient():
             return x * x
 
         @staticmethod
-        def gradients(ctx, g):
-            return 2 * ctx.saved_tensors[0] * g, None
+        def gradients(ctx, saved, g):
+            return 2 * saved[0] * g, None
 
     Square._bind("square")
     x = torch.tensor(3.0, requires_grad=True)
@@ -51,6 +51,11 @@ def test_a_second_derivative_is_refused_whatever_the_incoming_gradient():
     assert float(dx.detach()) == 6.0 and dx.requires_grad
     with pytest.raises(nv.SpmiError, match="square has no second derivative"):
         torch.autograd.grad(x + dx.square(), x)
+    from torch.utils.checkpoint import checkpoint  # (it hands out what was saved once)
+
+    (dx,) = torch.autograd.grad(checkpoint(lambda v: Square.apply(v, None), x, use_reentrant=False), x, create_graph=True)
+    with pytest.raises(nv.SpmiError, match="second derivative"):
+        dx.backward()
     g = torch.ones((), requires_grad=True)
     (dx,) = torch.autograd.grad(Square.apply(x, None), x, g, create_graph=True)
     with pytest.raises(nv.SpmiError, match="second derivative"):

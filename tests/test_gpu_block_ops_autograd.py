@@ -58,3 +58,36 @@ def test_a_recorded_backward_pass_is_an_ordinary_gradient(dev):
     ops.layer_norm(x, w).sum().backward(create_graph=True)
     assert torch.equal(x.grad, want[0]) and torch.equal(w.grad, want[1])
     x.grad = w.grad = None
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_under_activation_checkpointing(dev, dtype):
+    """Forward runs again before the backward pass: the same gradients to the bit."""
+    from torch.utils.checkpoint import checkpoint
+
+    gates, h0 = rand(40, 3, 16).to(dtype).requires_grad_(), rand(3, 8, seed=1).requires_grad_()
+    w = rand(8, seed=2).requires_grad_()
+
+    def block(g, s, v):
+        h, last = ops.gated_scan(g, s)
+        return ops.layer_norm(h, v), last
+
+    def grads(outs):
+        return torch.autograd.grad(outs[0].float().sum() + outs[1].sum(), (gates, h0, w))
+
+    want = grads(block(gates, h0, w))
+    got = grads(checkpoint(block, gates, h0, w, use_reentrant=False))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_states_may_move_on_before_the_backward_pass(dev, dtype):
+    """The start of a scan is a row of the node memory that later steps overwrite: what the backward pass needs
+    of it was taken in the forward pass, or the change is noticed."""
+    gates, memory = rand(30, 3, 16).to(dtype).requires_grad_(), rand(3, 8, seed=1)
+    (want,) = torch.autograd.grad(ops.gated_scan(gates, memory)[1].sum(), gates)
+    last = ops.gated_scan(gates, memory)[1]
+    ops.gated_step(rand(3, 16, seed=2), memory)
+    with pytest.raises(RuntimeError, match="modified"):
+        torch.autograd.grad(last.sum(), gates)
+    assert want.shape == gates.shape
