@@ -546,8 +546,11 @@ class GLRU(SequentialDecoder):
             x = torch.where(active[..., None], x, torch.zeros((), dtype=x.dtype, device=x.device))
         last = []
         for k in range(self.n_layers):
-            start = mem.layer(k) if whole else mem.memory[k].index_select(0, ids) if ids is not None \
-                else mem.memory[k][:n].clone()
+            if whole:
+                # not adopted below, the table stays in use: a later step may write it before this backward pass
+                start = mem.layer(k) if self.training_mode else mem.layer(k).clone()
+            else:
+                start = mem.memory[k][:n].clone() if ids is None else mem.memory[k].index_select(0, ids)
             gates = self.base_model.gates(x.reshape(t * n, x.shape[2]), k).reshape(t, n, 2 * self.hidden_d)
             x, end = ops.gated_scan(gates, start, active)
             last.append(end.detach())

@@ -105,3 +105,24 @@ def test_bfloat16_serving_in_8_bits(dev):
         out = dec((x[0], torch.arange(9)))
         assert out.shape == (9, 1) and out.dtype == torch.bfloat16 and bool(out.isfinite().all())
         assert dec.forward_sequence(x).shape == (2, 9, 1)
+
+
+@pytest.mark.parametrize("n", [9, 5])
+def test_a_sequence_that_leaves_the_memory_alone(dev, n):
+    """In eval mode the memory stays as it is; steps that move it on before the sequence's backward pass do not
+    reach what that pass uses."""
+    dec = make()
+    dec.train(False)
+    dec.eval_mode()
+    x = torch.randn(4, n, 12, device=dev)
+    state = dec.memory_h.memory.clone()
+    leaf = next(dec.base_model.parameters())
+    (want,) = torch.autograd.grad(dec.forward_sequence(x).sum(), leaf)
+    out = dec.forward_sequence(x)
+    assert torch.equal(dec.memory_h.memory, state)
+    dec.train_mode()
+    with torch.no_grad():
+        dec((x[0], torch.arange(n)))
+    assert not torch.equal(dec.memory_h.memory, state)
+    (got,) = torch.autograd.grad(out.sum(), leaf)
+    assert torch.equal(got, want)
