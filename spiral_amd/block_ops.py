@@ -207,7 +207,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     """(x - mean) / sqrt(variance + eps) * weight + bias over the last dimension of x [..., D],
     differentiable in x, weight and bias.  x: float32 or bfloat16 of any strides, D from 1 to 16384;
     weight and bias: [D] in either type, or None.  Statistics and gradient sums are float32; the
-    gradients of weight and bias are added up in a fixed order (the same bits every time)."""
+    gradients of weight and bias are added up in a fixed order (the same bits every time).  There is
+    no second derivative and no forward mode; a call that would need one is refused."""
     code = _code(x, "layer_norm: x")
     if x.dim() < 1 or not 1 <= x.shape[-1] <= LAYER_NORM_MAX_WIDTH:
         _refuse(f"layer_norm: the last dimension of x must be 1 to {LAYER_NORM_MAX_WIDTH}, got {tuple(x.shape)}")
@@ -312,7 +313,10 @@ def gated_scan(gates: torch.Tensor, h0: Optional[torch.Tensor] = None, active: O
     bool [T, N] ([N, T]); where it is False the node's state passes the step unchanged, its gates
     are not used (they may hold anything) and receive a zero gradient.  A node that joins late or a
     sequence that ends early is described by it.  Returns the states [T, N, H] ([N, T, H]) in the
-    type of `gates` and the last state [N, H] in float32 (h0 where no step is active)."""
+    type of `gates` and the last state [N, H] in float32 (h0 where no step is active).
+
+    The gradient is that of float32 states whatever the type of `gates`: with bfloat16, a tracked call keeps
+    a float32 state for every 4 steps (2 where the channels are few) besides."""
     code = _code(gates, "gated_scan: gates")
     if gates.dim() != 3 or gates.shape[2] < 2 or gates.shape[2] % 2:
         _refuse(f"gated_scan: gates must be [T, N, 2H], got {tuple(gates.shape)}")
@@ -411,7 +415,7 @@ def quantize_rows_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     float32 of its leading shape, x = q * scale to within half a scale.  With m the row's largest
     magnitude (at least 2^-120), scale = m / 127 and q = rint(x * (127 / m)), each operation rounded
     to float32.  A row with a value that is not finite gets q = 0 and scale = NaN.  Applied to a
-    weight [N, K] this gives the arguments of `linear_int8`."""
+    weight [N, K] this gives the arguments of `linear_int8`.  Both results are constants to autograd."""
     code = _code(x, "quantize_rows_int8: x")
     if x.dim() < 1 or not 1 <= x.shape[-1] <= INT8_MAX_INNER:
         _refuse(f"quantize_rows_int8: the last dimension of x must be 1 to {INT8_MAX_INNER}, got {tuple(x.shape)}")
@@ -433,7 +437,7 @@ def linear_int8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     (`quantize_rows_int8`), the sums over K are exact, scales, bias and activation (None, "relu" or
     "leaky_relu" with `slope`) follow in float32, and the result [..., N] is rounded once to
     `out_dtype` (default: x's type).  weight: int8 [N, K], weight_scale: float32 [N]; K up to 131072.
-    For serving: there is no backward pass, and a call that would need one is refused."""
+    A result depends on its own row of x and its own channel alone, to the bit.  For serving: there is no backward pass, and a call that would need one is refused."""
     code = _code(x, "linear_int8: x")
     if weight.dim() != 2 or weight.dtype != torch.int8:
         _refuse(f"linear_int8: weight must be int8 [N, K], got {weight.dtype} {tuple(weight.shape)}")

@@ -8,7 +8,8 @@
 // computed from it: the mean first and then the centred squares (a single pass over E[x^2] would
 // cancel for rows whose mean is large against their deviation), all in float32 for either storage
 // type.  G neighbouring lanes own a row, four values of R vectors each: G = 8..64 for widths up to
-// 2048, a workgroup of 256 or 1024 threads beyond (16384 at most).
+// 2048, a workgroup of 256 or 1024 threads beyond (16384 at most; the bfloat16 backward kernel of more than
+// 8192 keeps four of its 132 registers in scratch).
 //
 // The gradients of w and b are column sums over all rows.  A lane sees the same columns in every
 // row its group visits, so it adds them up in registers; the groups of a workgroup meet in LDS,
