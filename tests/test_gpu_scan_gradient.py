@@ -104,3 +104,69 @@ def test_step_and_scan_train_alike(dev):
     (a,) = torch.autograd.grad(out, one, g[0].float())
     (b,) = torch.autograd.grad(ops.gated_scan(two, h0)[0], two, g)
     assert torch.equal(a, b[0])
+
+
+@pytest.mark.parametrize("t,n,h", [(11, 40, 20), (300, 2, 64), (3000, 1, 24)])
+def test_captured_and_replayed(dev, t, n, h):
+    """Forward and backward of bfloat16 sequences in one graph, in each layout: every replay on new inputs
+    against the eager result, with eager work between the replays."""
+    gates, h0, g, g_last = inputs(t, n, h, BF16)
+    on = torch.rand(t, n, generator=torch.Generator().manual_seed(1)).to(dev) < 0.8
+    leaf, start = gates.clone().requires_grad_(), h0.clone().requires_grad_()
+
+    def work(leaf, start):
+        h, last = ops.gated_scan(leaf, start, on)
+        return [h.detach(), last.detach(), *torch.autograd.grad((h, last), (leaf, start), (g, g_last))]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work(leaf, start)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = work(leaf, start)
+    for k in range(3):
+        new, new0 = inputs(t, n, h, BF16, seed=50 + k)[:2]
+        with torch.no_grad():
+            leaf.copy_(new)
+            start.copy_(new0)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = work(new.requires_grad_(), new0.requires_grad_())
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_offsets_past_32_bits_of_many_nodes(dev, dtype):
+    """Gates of more than 2^31 values: the last nodes come out as they do alone."""
+    t, n, h = 5, (1 << 31) // (5 * 128) + 9, 64
+    tail = inputs(t, 8, h, dtype)
+    gates = torch.zeros(t, n, 2 * h, dtype=dtype, device=dev)
+    gates[:, -8:] = tail[0]
+    leaf, short = gates.requires_grad_(), tail[0].clone().requires_grad_()
+    last = ops.gated_scan(leaf)[1]
+    g_last = torch.zeros_like(last)
+    g_last[-8:] = tail[3]
+    (dgates,) = torch.autograd.grad(last, leaf, g_last)
+    (want,) = torch.autograd.grad(ops.gated_scan(short)[1], short, tail[3])
+    assert torch.equal(dgates[:, -8:], want) and not dgates[:, :8].any()
+
+
+def test_offsets_past_32_bits_of_many_steps(dev):
+    """A sequence of more than 2^31 values, split over workgroups: the gradient of its last steps is that of
+    a short one from their first state on, up to the roundings of joined maps (16 u a step, 40 steps)."""
+    t, h = (1 << 31) // 128 + 40, 64
+    gates = torch.zeros(t, 1, 2 * h, device=dev)
+    gates[-200:] = inputs(200, 1, h, F32)[0]
+    leaf = gates.requires_grad_()
+    hs, last = ops.gated_scan(leaf)
+    g_last = torch.ones(1, h, device=dev)
+    start, short = hs[-41].detach().clone(), gates[-40:].detach().clone().requires_grad_()
+    (dgates,) = torch.autograd.grad(last, leaf, g_last)
+    del hs
+    (want,) = torch.autograd.grad(ops.gated_scan(short, start)[1], short, g_last)
+    got = dgates[-40:]
+    # dz cancels: the states (of about 4) are off by 16 u a step, carried on
+    allowed = 40 * 16 * U * (want.abs() + (want[..., h:].abs() * 8).repeat(1, 1, 2)) + 1e-30
+    assert bool(((got - want).abs() <= allowed).all())
