@@ -648,9 +648,10 @@ __global__ __launch_bounds__(RowsShape<KP>::NW * 64, 2) void rows_i8_kernel(Rows
     for (int k = 0; k < KS; ++k)
       acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(
           xa[k], *reinterpret_cast<const i32x4*>(slice + lr * SK + k * 32 + lh * 16), acc, 0, 0, 0);
-    if constexpr (KS >= 4) {
-      // Four operands ahead of the products that take them: left to itself the compiler reads each when it is
-      // needed (100003 x 512 -> 1024 takes 157 us so, and 149 with the reads ahead).
+    if constexpr (KS > 8) {
+      // Four operands ahead of the products that take them.  Left to itself the compiler reads each of the 16 when
+      // it is needed: 100003 x 512 -> 1024 takes 156 us so, and 148 with the reads ahead.  The shorter rows' kernels
+      // have more waves to cover the wait, and the order costs them (20863 x 182 -> 3265 in bfloat16 98 us, 91 without).
       __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
       for (int k = 0; k < KS - 4; ++k) {
