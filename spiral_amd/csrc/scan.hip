@@ -375,7 +375,8 @@ __global__ __launch_bounds__(kThreads, S > 1 ? 4 : 1) void scan_bwd_kernel(ScanA
       for (int i = 0; i < L; ++i) raw_g[i] = take<STREAM, TINY>(g + step_at(u0 + strand * L + i) * p.g_t, at.left);
     }
     if constexpr (!MAPS) {
-      const int64_t group = (steps - 1 - (u0 + strand * L)) / L;  // strands past the end: not above zero
+      // (a strand past the end of its split reads what is before an earlier group, or h0, and does not use it)
+      const int64_t group = (steps - 1 - (u0 + strand * L)) / L;
       const float* const src = group > 0 ? p.before + (group - 1) * p.before_g : p.h0;
       raw_s = held<float>{0.0f, 0.0f, 0.0f, 0.0f};
       if (src) raw_s = take<STREAM, TINY>(src + at.n * (group > 0 ? p.before_n : p.h0_n) + at.c, at.left);
